@@ -1,0 +1,321 @@
+// Decoding with drafted tokens: what stands around the model's pass over a tree of guesses per request.
+//
+// A request s has lengths[s] tokens in the cache and brings the rows cu_nodes[s] .. cu_nodes[s + 1] of the step; row i hangs on
+// row parents[i] < i of its own request, or on the text (-1).  Row 0 is the token that is decided already.
+//
+//   draft_tables   page lists and lengths -> block table, cache slots, positions, visibility bits   (before the pass)
+//   accept_drafts  logits -> the model's choice at every row, the longest path that agrees with it  (after the pass)
+//   keep_accepted  the cache rows of that path move next to the text, in every layer                (after that)
+//
+// All three read lengths that an earlier kernel of the same stream may have written, so nothing has to come back to the host
+// between two steps.
+#include "common.cuh"
+
+namespace {
+
+constexpr int MAX_NODES = 256;       // rows of a tree: one thread each, eight words of visibility bits
+constexpr int TABLE_THREADS = 256;
+
+// One block per request and slice of its block-table row; the first slice also does the request's rows.
+//
+// Depths and ancestors by pointer doubling: seen_i = {i} and up_i = parent_i at first; a round sets seen_i |= seen_{up_i},
+// up_i = up_{up_i}, after which seen_i covers twice as many steps towards the root.  log2(n) rounds, and the depth is the number of
+// bits less one.  What bounds it: a launch and a chain of two loads (cu_pages, then the pages) for one request, the stores of the
+// table for many.
+__global__ void __launch_bounds__(TABLE_THREADS)
+draft_tables_kernel(const int* lengths, const int* cu_nodes, const int* parents, const int* pages, const int* cu_pages, int page_size,
+                    int* __restrict__ block_table, int width, int* __restrict__ slots, int* __restrict__ positions,
+                    int* __restrict__ token_seq, int* __restrict__ ctx_len, int* __restrict__ ancestors, int words) {
+    __shared__ int s_up[MAX_NODES];
+    __shared__ unsigned int s_seen[MAX_NODES / 32][MAX_NODES];
+    pdl_wait();
+    pdl_launch();
+    const int s = blockIdx.x, tid = threadIdx.x;
+    const int first = cu_nodes[s], n = cu_nodes[s + 1] - first;
+    const int p0 = cu_pages[s], held = cu_pages[s + 1] - p0;
+    const int len = lengths[s];
+    const int* mine = pages + p0;
+    for (int c = blockIdx.y * TABLE_THREADS + tid; c < width; c += gridDim.y * TABLE_THREADS)
+        block_table[(size_t)s * width + c] = c < held ? max(mine[c], 0) : 0;
+    if (blockIdx.y != 0) return;
+    if (tid == 0) ctx_len[s] = len + n;
+    const int most = parents ? min(n, 32 * words) : n;         // rows past the bits take no part: they are stored nowhere
+    if (parents) {
+        const bool on = tid < most;
+        int up = on ? parents[first + tid] : -1;
+        if (up >= tid || up < 0) up = -1;                      // a parent comes before its children; anything else is none
+        unsigned int seen[MAX_NODES / 32];
+#pragma unroll
+        for (int w = 0; w < MAX_NODES / 32; ++w) seen[w] = w == tid >> 5 ? 1u << (tid & 31) : 0u;
+        for (int reach = 1; reach < most; reach <<= 1) {
+            s_up[tid] = up;
+#pragma unroll
+            for (int w = 0; w < MAX_NODES / 32; ++w)
+                if (w < words) s_seen[w][tid] = seen[w];
+            __syncthreads();
+            if (up >= 0) {
+#pragma unroll
+                for (int w = 0; w < MAX_NODES / 32; ++w)
+                    if (w < words) seen[w] |= s_seen[w][up];
+                up = s_up[up];
+            }
+            __syncthreads();
+        }
+        if (on) {
+            int depth = -1;
+#pragma unroll
+            for (int w = 0; w < MAX_NODES / 32; ++w)
+                if (w < words) {
+                    depth += __popc(seen[w]);
+                    ancestors[(size_t)(first + tid) * words + w] = (int)seen[w];
+                }
+            positions[first + tid] = len + depth;
+        }
+    }
+    for (int i = tid; i < n; i += TABLE_THREADS) {
+        const int place = len + i, p = place / page_size;
+        const int page = i < most && place >= 0 && p < held ? mine[p] : -1;
+        slots[first + i] = page >= 0 ? page * page_size + place % page_size : -1;
+        token_seq[first + i] = s;
+        if (!parents) positions[first + i] = place;
+        else if (i >= most) positions[first + i] = len;
+        if (ancestors && (!parents || i >= most))              // a chain sees all rows before it
+            for (int w = 0; w < words; ++w) {
+                const int left = i + 1 - 32 * w;
+                ancestors[(size_t)(first + i) * words + w] = parents || left <= 0 ? 0 : left >= 32 ? -1 : (int)((1u << left) - 1u);
+            }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------- acceptance
+// (value, index) of the larger value, the lower index among equals; an index of -1 stands for nothing yet.  NaN never wins.
+__device__ __forceinline__ void better(float& v, int& i, float ov, int oi) {
+    if (oi >= 0 && (i < 0 || ov > v || (ov == v && oi < i))) { v = ov; i = oi; }
+}
+
+constexpr int SCAN_THREADS = 256;
+
+// The largest logit of one slice of a row.  Rows of an odd vocabulary start anywhere, so a slice is cut at 16-byte boundaries of
+// memory: single loads up to the first and from the last, vector loads in between, four in flight per thread.
+__global__ void __launch_bounds__(SCAN_THREADS)
+accept_scan_kernel(const float* logits, long long ld, int V, int slices, float* __restrict__ part_val, int* __restrict__ part_idx) {
+    __shared__ float s_val[SCAN_THREADS / 32];
+    __shared__ int s_idx[SCAN_THREADS / 32];
+    pdl_wait();
+    pdl_launch();
+    const int r = blockIdx.x / slices, sl = blockIdx.x % slices, tid = threadIdx.x;
+    const float* row = logits + (size_t)r * ld;
+    const int skew = (int)(((uintptr_t)row >> 2) & 3);                 // elements past a 16-byte boundary
+    const int quads = (V + skew + 3) / 4;                              // 16-byte pieces that the row touches
+    const int per = (quads + slices - 1) / slices;
+    const int q0 = min(quads, sl * per), q1 = min(quads, q0 + per);
+    const float4* vec = reinterpret_cast<const float4*>(row - skew);
+    float best = -INFINITY;
+    int idx = -1;
+    auto take = [&](float v, int i) {
+        if (v > best || (v == best && idx < 0)) { best = v; idx = i; }          // i only rises within a thread
+    };
+    const int whole0 = skew ? max(q0, 1) : q0;                         // pieces that lie in the row as a whole
+    const int whole1 = (V + skew) % 4 ? min(q1, quads - 1) : q1;
+    if (skew && q0 == 0 && tid < 4 && tid >= skew && tid - skew < V) take(row[tid - skew], tid - skew);
+    int q = whole0 + tid;
+    for (; q + 3 * SCAN_THREADS < whole1; q += 4 * SCAN_THREADS) {
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = vec[q + u * SCAN_THREADS];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = 4 * (q + u * SCAN_THREADS) - skew;
+            take(v[u].x, i); take(v[u].y, i + 1); take(v[u].z, i + 2); take(v[u].w, i + 3);
+        }
+    }
+    for (; q < whole1; q += SCAN_THREADS) {
+        const float4 v = vec[q];
+        const int i = 4 * q - skew;
+        take(v.x, i); take(v.y, i + 1); take(v.z, i + 2); take(v.w, i + 3);
+    }
+    if (whole1 < q1 && q1 == quads && quads - 1 >= whole0 && tid < 4) {     // the last piece, where it reaches past the row
+        const int i = 4 * (quads - 1) - skew + tid;
+        if (i < V) take(row[i], i);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) better(best, idx, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, idx, o));
+    if ((tid & 31) == 0) { s_val[tid >> 5] = best; s_idx[tid >> 5] = idx; }
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 1; w < SCAN_THREADS / 32; ++w) better(best, idx, s_val[w], s_idx[w]);
+        part_val[(size_t)r * slices + sl] = best;
+        part_idx[(size_t)r * slices + sl] = idx;
+    }
+}
+
+// One block per request: the slices of every row meet (a warp per row), then child[p] = the lowest row that hangs on p and holds
+// the token chosen there, and one thread follows the children from row 0.
+__global__ void __launch_bounds__(MAX_NODES)
+accept_walk_kernel(const float* part_val, const int* part_idx, int slices, int* chosen, const int* tokens, const int* parents,
+                   const int* cu_nodes, const int* lengths, int* __restrict__ path, int depth, int* __restrict__ accepted,
+                   int* __restrict__ next_token, int* __restrict__ new_lengths) {
+    __shared__ int s_chosen[MAX_NODES], s_child[MAX_NODES];
+    pdl_wait();
+    pdl_launch();
+    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int first = cu_nodes[s], n = cu_nodes[s + 1] - first;
+    if (slices > 0) {
+        for (int i = warp; i < n; i += MAX_NODES / 32) {
+            float best = -INFINITY;
+            int idx = -1;
+            for (int k = lane; k < slices; k += 32)
+                better(best, idx, part_val[(size_t)(first + i) * slices + k], part_idx[(size_t)(first + i) * slices + k]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+                better(best, idx, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, idx, o));
+            if (lane == 0) {
+                chosen[first + i] = max(idx, 0);                         // a row without a number takes token 0
+                if (i < MAX_NODES) s_chosen[i] = max(idx, 0);
+            }
+        }
+    } else if (tid < n) {
+        s_chosen[tid] = chosen[first + tid];
+    }
+    s_child[tid] = MAX_NODES;
+    __syncthreads();
+    if (tid > 0 && tid < n) {
+        const int up = parents[first + tid];
+        if (up >= 0 && up < tid && tokens[first + tid] == s_chosen[up]) atomicMin(&s_child[up], tid);
+    }
+    __syncthreads();
+    int* mine = path + (size_t)s * depth;
+    if (tid == 0) {
+        int count = 0, last = 0;
+        for (int at = n > 0 ? 0 : MAX_NODES; at < MAX_NODES && count < depth; at = s_child[at]) {
+            mine[count++] = at;
+            last = at;
+        }
+        accepted[s] = count;
+        next_token[s] = count ? s_chosen[last] : -1;
+        new_lengths[s] = lengths[s] + count;
+        for (int k = count; k < depth; ++k) mine[k] = -1;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------- kept rows
+// Row `lengths + path[k]` of a request moves to `lengths + k`, for every plane (keys or values of a layer) and head.  A thread owns
+// one column of U bytes and moves the path's rows in rising order, eight at a time: all eight are loaded before the first is
+// stored, and since path[k] >= k and rises, no row is overwritten before it has been read.  So threads need not wait for one
+// another, and source and destination may overlap.
+template <typename U>
+__global__ void __launch_bounds__(128)
+keep_accepted_kernel(U* planes, long long plane_stride, int n_planes, int pages, int heads, int page_size, int row_units,
+                     const int* block_table, int bt_stride, int width, const int* lengths, const int* path, int depth,
+                     const int* accepted) {
+    constexpr int AT_ONCE = 8;
+    pdl_wait();
+    pdl_launch();
+    const int s = blockIdx.y;
+    const int count = min(accepted[s], depth);
+    if (count <= 1 && !(count == 1 && path[(size_t)s * depth] != 0)) return;
+    const int len = lengths[s];
+    const int per_plane = heads * row_units;
+    const long long total = (long long)n_planes * per_plane;
+    // the row of the cache that holds a position, or -1 where the request holds no page for it
+    auto row_of = [&](int place) -> long long {
+        const int p = place / page_size;
+        if (place < 0 || p >= width) return -1;
+        const int page = block_table[(size_t)s * bt_stride + p];
+        if (page < 0 || page >= pages) return -1;
+        return (long long)page * heads * page_size + place % page_size;
+    };
+    for (long long c = (long long)blockIdx.x * blockDim.x + threadIdx.x; c < total; c += (long long)gridDim.x * blockDim.x) {
+        const int plane = (int)(c / per_plane), rest = (int)(c % per_plane), h = rest / row_units, u = rest % row_units;
+        U* base = planes + (size_t)plane * plane_stride + (size_t)h * page_size * row_units + u;
+        for (int k0 = 0; k0 < count; k0 += AT_ONCE) {
+            U v[AT_ONCE];
+            long long to[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                to[i] = -1;
+                if (k0 + i < count) {
+                    const int from = path[(size_t)s * depth + k0 + i];
+                    if (from > k0 + i) {                       // row 0 and what else stands in its place already stays
+                        const long long a = row_of(len + from), b = row_of(len + k0 + i);
+                        if (a >= 0 && b >= 0) { v[i] = base[(size_t)a * row_units]; to[i] = b; }
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i)
+                if (to[i] >= 0) base[(size_t)to[i] * row_units] = v[i];
+        }
+    }
+}
+
+}  // namespace
+
+MLLM_EXPORT int mllm_draft_max_nodes() { return MAX_NODES; }
+
+// parents may be null (every row follows the one before it), ancestors then too.
+MLLM_EXPORT int mllm_draft_tables(const int* lengths, const int* cu_nodes, const int* parents, const int* pages, const int* cu_pages,
+                                  int S, int page_size, int* block_table, int width, int* slots, int* positions, int* token_seq,
+                                  int* ctx_len, int* ancestors, int words, cudaStream_t stream) {
+    if (S <= 0) return 0;
+    if (page_size <= 0 || width <= 0) return mllm_fail(1, "draft_tables: pages of %d tokens, a table of %d columns", page_size, width);
+    if ((parents && !ancestors) || (ancestors && (words <= 0 || words > MAX_NODES / 32)))
+        return mllm_fail(1, "draft_tables: a tree needs 1 to %d words of bits per row, got %d", MAX_NODES / 32, ancestors ? words : 0);
+    // a block writes up to 1,024 columns of the table
+    const int slices = (width + 4 * TABLE_THREADS - 1) / (4 * TABLE_THREADS);
+    if (slices > 65535) return mllm_fail(1, "draft_tables: a table of %d columns is more than one launch takes", width);
+    MLLM_CUDA(mllm_launch(draft_tables_kernel, dim3(S, slices), dim3(TABLE_THREADS), 0, stream, true, lengths, cu_nodes, parents,
+                          pages, cu_pages, page_size, block_table, width, slots, positions, token_seq, ctx_len, ancestors, words));
+    return 0;
+}
+
+// Slices into which a row of V logits is cut: enough blocks for every SM, no slice under 2,048 logits.
+MLLM_EXPORT int mllm_accept_slices(int rows, int V) {
+    const int want = rows > 0 ? (4736 + rows - 1) / rows : 1;          // 32 blocks per SM
+    const int most = (V + 2047) / 2048;
+    return want < most ? (want < 1 ? 1 : want) : (most < 1 ? 1 : most);
+}
+
+// logits null: `chosen` is read instead of written.  part_val, part_idx: rows x slices of scratch.
+MLLM_EXPORT int mllm_accept_drafts(const float* logits, long long ld, int T, int V, int slices, float* part_val, int* part_idx,
+                                   int* chosen, const int* tokens, const int* parents, const int* cu_nodes, const int* lengths,
+                                   int S, int* path, int depth, int* accepted, int* next_token, int* new_lengths,
+                                   cudaStream_t stream) {
+    if (S <= 0) return 0;
+    if (depth <= 0) return mllm_fail(1, "accept_drafts: paths of %d rows", depth);
+    if (logits && T > 0) {
+        if (V <= 0 || slices <= 0 || (long long)T * slices > 0x7fffffffLL)
+            return mllm_fail(1, "accept_drafts: vocabulary %d, %d rows in %d slices", V, T, slices);
+        MLLM_CUDA(mllm_launch(accept_scan_kernel, dim3(T * slices), dim3(SCAN_THREADS), 0, stream, true, logits, ld, V, slices,
+                              part_val, part_idx));
+    }
+    MLLM_CUDA(mllm_launch(accept_walk_kernel, dim3(S), dim3(MAX_NODES), 0, stream, true, (const float*)part_val, (const int*)part_idx,
+                          logits ? slices : 0, chosen, tokens, parents, cu_nodes, lengths, path, depth, accepted, next_token,
+                          new_lengths));
+    return 0;
+}
+
+// planes: n_planes x [pages, heads, page_size, row_bytes], plane_bytes apart.
+MLLM_EXPORT int mllm_keep_accepted(void* planes, long long plane_bytes, int n_planes, int pages, int heads, int page_size,
+                                   int row_bytes, const int* block_table, int bt_stride, int width, const int* lengths,
+                                   const int* path, int depth, const int* accepted, int S, cudaStream_t stream) {
+    if (S <= 0 || n_planes <= 0) return 0;
+    if (depth <= 0 || page_size <= 0 || heads <= 0 || row_bytes <= 0 || S > 65535)
+        return mllm_fail(1, "keep_accepted: paths of %d rows, %d heads, pages of %d, rows of %d bytes, %d requests", depth, heads,
+                         page_size, row_bytes, S);
+#define GO(U)                                                                                                                     \
+    do {                                                                                                                          \
+        const long long cols = (long long)n_planes * heads * (row_bytes / (int)sizeof(U));                                        \
+        const int grid = (int)((cols + 127) / 128 < 2048 ? (cols + 127) / 128 : 2048);                                            \
+        MLLM_CUDA(mllm_launch(keep_accepted_kernel<U>, dim3(grid, S), dim3(128), 0, stream, true, (U*)planes,                     \
+                              plane_bytes / (long long)sizeof(U), n_planes, pages, heads, page_size, row_bytes / (int)sizeof(U),  \
+                              block_table, bt_stride, width, lengths, path, depth, accepted));                                    \
+        return 0;                                                                                                                 \
+    } while (0)
+    if (row_bytes % 16 == 0 && (uintptr_t)planes % 16 == 0 && plane_bytes % 16 == 0) GO(uint4);
+    if (row_bytes % 4 == 0 && (uintptr_t)planes % 4 == 0 && plane_bytes % 4 == 0) GO(uint32_t);
+    if (row_bytes % 2 == 0 && (uintptr_t)planes % 2 == 0 && plane_bytes % 2 == 0) GO(uint16_t);
+#undef GO
+    return mllm_fail(1, "keep_accepted: rows of %d bytes", row_bytes);
+}

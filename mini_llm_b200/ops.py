@@ -9,6 +9,7 @@ tensor is not on a CUDA device, the call fails with an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from typing import Optional
 
@@ -116,6 +117,17 @@ def _signatures(lib):
                                  c_void_p, c_ll, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
         "mllm_attention_tiled_wide": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                       c_void_p, c_ll, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
+        "mllm_draft_max_nodes": [],
+        "mllm_draft_tables": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                              c_void_p, c_void_p, c_void_p, c_int, c_void_p],
+        "mllm_tree_attention": [c_void_p, c_ll, c_void_p, c_void_p, c_ll, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int,
+                                c_void_p, c_ll, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
+                                c_int, c_int, c_void_p],
+        "mllm_accept_slices": [c_int, c_int],
+        "mllm_accept_drafts": [c_void_p, c_ll, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                               c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+        "mllm_keep_accepted": [c_void_p, c_ll, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
+                               c_void_p, c_int, c_void_p],
         "mllm_rmsnorm": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_int, c_int, c_int, c_float,
                          c_float, c_float, c_int, c_void_p],
         "mllm_gated_recurrence_wide": [c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_void_p, c_void_p,
@@ -2335,6 +2347,186 @@ def _attend(impl, q, ldq, k_pages, v_pages, block_table, bt_stride, ctx, out, ld
     _call("mllm_attention_simt", q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
           bt_stride, ctx.token_seq.data_ptr(), ctx.positions.data_ptr(), out.data_ptr(), ldo, T, num_heads,
           num_kv_heads, head_dim, ps, float(scale), int(window or 0), _dt(q), _stream())
+
+
+# --------------------------------------------------------------------------- drafted tokens
+# A step may bring, for each of S requests, a tree of drafted tokens: the rows cu_nodes[s] .. cu_nodes[s + 1] of the step, at most
+# DRAFT_MAX_NODES of them.  Row 0 of a request is the token that is decided already, every other row names the row of its own request
+# that it hangs on (parents: an earlier row; -1: on the text itself).  Lengths, trees and results are int32 tensors on the device, so
+# that a step can follow the one before it without the host knowing how many tokens that one kept.  A request may bring no row.
+DRAFT_MAX_NODES = 256
+TREE_ATTN_TARGET_BLOCKS = 592      # blocks that a tree attention is cut into where its keys allow: four per SM
+
+
+def _request_ints(who: str, lengths, cu_nodes) -> int:
+    _cuda("lengths", lengths, torch.int32)
+    _cuda("cu_nodes", cu_nodes, torch.int32)
+    S = lengths.numel()
+    if cu_nodes.numel() != S + 1:
+        raise KernelError(f"{who}: {S} requests need {S + 1} starts of their rows, got {cu_nodes.numel()}")
+    return S
+
+
+def draft_tables(lengths, cu_nodes, parents, pages, cu_pages, page_size: int, *, block_table, slot_mapping, positions, token_seq,
+                 ctx_len, ancestors=None) -> None:
+    """What a step needs to know about its rows, made on the device from the requests' lengths and page lists.
+
+    ``lengths`` [S]: tokens of each request that are in the cache; ``cu_nodes`` [S + 1]: starts of the requests' rows;
+    ``parents`` [T], or None where every row follows the one before it (no limit on their number then); ``pages``,
+    ``cu_pages`` [S + 1]: the requests' page ids one after the other, in order of position (a negative id: given back).
+    Written: ``block_table`` [S, width] (zeros behind a request's pages), ``slot_mapping`` [T] (row i stands at place
+    length + i; -1, stored nowhere, where the request holds no page for it), ``positions`` [T] (length + depth in the
+    tree), ``token_seq`` [T], ``ctx_len`` [S] (length + rows) and ``ancestors`` [T, words]: bit b of word w says that row
+    32 w + b of the request is the row itself or on its way to the root.  Rows past 32 * words take no part: no slot, no bits."""
+    S = _request_ints("draft_tables", lengths, cu_nodes)
+    for name, t in (("pages", pages), ("cu_pages", cu_pages), ("block_table", block_table), ("slot_mapping", slot_mapping),
+                    ("positions", positions), ("token_seq", token_seq), ("ctx_len", ctx_len)):
+        _cuda(name, t, torch.int32)
+    T = slot_mapping.numel()
+    if block_table.dim() != 2 or block_table.shape[0] != S or cu_pages.numel() != S + 1 or ctx_len.numel() != S \
+            or positions.numel() != T or token_seq.numel() != T:
+        raise KernelError(f"draft_tables: the tables of {S} requests and {T} rows do not fit: block_table {tuple(block_table.shape)}, "
+                          f"cu_pages {cu_pages.numel()}, ctx_len {ctx_len.numel()}, positions {positions.numel()}, "
+                          f"token_seq {token_seq.numel()}")
+    words = 0
+    if ancestors is not None:
+        _cuda("ancestors", ancestors, torch.int32)
+        if ancestors.dim() != 2 or ancestors.shape[0] != T or not 1 <= ancestors.shape[1] <= DRAFT_MAX_NODES // 32:
+            raise KernelError(f"draft_tables: ancestors must be [{T}, 1 to {DRAFT_MAX_NODES // 32}], got {tuple(ancestors.shape)}")
+        words = ancestors.shape[1]
+    if parents is not None:
+        _cuda("parents", parents, torch.int32)
+        if parents.numel() != T or ancestors is None:
+            raise KernelError(f"draft_tables: a tree needs a parent for each of its {T} rows, and ancestors to write")
+    if page_size <= 0:
+        raise KernelError(f"draft_tables: pages of {page_size} tokens")
+    _call("mllm_draft_tables", lengths.data_ptr(), cu_nodes.data_ptr(), None if parents is None else parents.data_ptr(),
+          pages.data_ptr(), cu_pages.data_ptr(), S, int(page_size), block_table.data_ptr(), block_table.shape[1],
+          slot_mapping.data_ptr(), positions.data_ptr(), token_seq.data_ptr(), ctx_len.data_ptr(),
+          None if ancestors is None else ancestors.data_ptr(), words, _stream())
+
+
+@functools.lru_cache(maxsize=1024)
+def tree_plan(float32: bool, S: int, num_heads: int, num_kv_heads: int, max_nodes: int, max_length: int):
+    """(query rows per block, blocks that share a key/value head's rows, spans of a request's keys) of a tree attention: the
+    smallest tile that holds a tree's rows, and as many spans as it takes to fill the GPU, none under 64 keys."""
+    rows = max(1, max_nodes * (num_heads // num_kv_heads))
+    tile = next((t for t in ((4, 8, 16) if float32 else (16, 32)) if rows <= t), 64)
+    tiles = min(-(-rows // tile), 65535 // num_kv_heads)
+    most = -(-(max_length + max_nodes) // 64)
+    return tile, tiles, max(1, min(-(-TREE_ATTN_TARGET_BLOCKS // (S * num_kv_heads * tiles)), most, 64))
+
+
+def tree_attention(q, k_pages, v_pages, block_table, lengths, cu_nodes, ancestors, out, *, num_heads, num_kv_heads, head_dim, scale,
+                   max_nodes: Optional[int] = None, max_length: Optional[int] = None) -> None:
+    """Attention of the rows of trees over the cache: a row sees its request's first ``lengths[s]`` places and those of the rows
+    whose bit is set in its words of ``ancestors`` (``draft_tables`` writes them; row i's keys and values stand at place
+    length + i).  A row that sees nothing gives zeros; what masked places hold, infinities and NaN too, has no effect.
+
+    q [T, heads * head_dim] and out (rows contiguous, any stride), pages [num_pages, kv_heads, page_size, head_dim],
+    block_table [S, width].  ``max_nodes`` and ``max_length``: the most rows and the longest text that a request brings, where the
+    host knows them; they only decide how the work is cut (without them: what ancestors and block_table can hold)."""
+    global launches
+    S = _request_ints("tree_attention", lengths, cu_nodes)
+    _cuda("q", q, contiguous=False)
+    _cuda("k_pages", k_pages, q.dtype)
+    _cuda("v_pages", v_pages, q.dtype)
+    _cuda("out", out, q.dtype, contiguous=False)
+    _cuda("block_table", block_table, torch.int32, contiguous=False)
+    _cuda("ancestors", ancestors, torch.int32)
+    ldq, ldo, bt_stride = _rows("q", q), _rows("out", out), _rows("block_table", block_table)
+    T, dt = q.shape[0], _dt(q)
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise KernelError(f"tree_attention: pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+    P, Hkv, ps, dh = k_pages.shape
+    if Hkv != num_kv_heads or dh != head_dim or q.shape[1] != num_heads * head_dim or tuple(out.shape) != tuple(q.shape) \
+            or num_heads % num_kv_heads:
+        raise KernelError("tree_attention: head counts or sizes do not fit the pages")
+    if head_dim % 16 != 0 or not (16 <= head_dim <= 256):
+        raise KernelError(f"tree_attention: head size {head_dim} is not a multiple of 16 in 16..256")
+    if block_table.shape[0] != S:
+        raise KernelError(f"tree_attention: block_table {tuple(block_table.shape)} for {S} requests")
+    if ancestors.dim() != 2 or ancestors.shape[0] != T or not 1 <= ancestors.shape[1] <= DRAFT_MAX_NODES // 32:
+        raise KernelError(f"tree_attention: ancestors must be [{T}, 1 to {DRAFT_MAX_NODES // 32}], got {tuple(ancestors.shape)}")
+    if T == 0 or S == 0:
+        return
+    width, words = block_table.shape[1], ancestors.shape[1]
+    tile, tiles, splits = tree_plan(dt == F32, S, num_heads, num_kv_heads, min(T, 32 * words if max_nodes is None else int(max_nodes)),
+                                    width * ps if max_length is None else min(int(max_length), width * ps))
+    part_o = part_ml = None
+    if splits > 1:
+        part = _scratch("tree_attn", q.device, splits * T * num_heads * (head_dim + 2))
+        part_o = part.data_ptr()
+        part_ml = part_o + 4 * splits * T * num_heads * head_dim
+    attention_launches["tree"] = attention_launches.get("tree", 0) + 1
+    _call("mllm_tree_attention", q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), P, block_table.data_ptr(), bt_stride, width,
+          lengths.data_ptr(), cu_nodes.data_ptr(), ancestors.data_ptr(), words, out.data_ptr(), ldo, part_o, part_ml, T, S, num_heads,
+          num_kv_heads, head_dim, ps, float(scale), tile, tiles, splits, dt, _stream())
+    if splits > 1:
+        launches += 1           # the kernel in which the spans meet
+
+
+def accept_drafts(tokens, parents, cu_nodes, lengths, *, chosen, path, accepted, next_token, new_lengths, logits=None) -> None:
+    """The longest path of each request's tree that agrees with the model.
+
+    ``chosen`` [T] is the token that the model puts after each row: with ``logits`` [T, vocab] (32-bit, rows contiguous) it is
+    written, the index of the largest (the lowest among equals); without them it is read, e.g. what ``sample`` drew.  The path
+    starts at row 0 of the request and goes on to the lowest row that hangs on its last one and whose ``tokens`` entry is what was
+    chosen there.  Written: ``path`` [S, depth] (rows within the request, -1 behind the end; a path is cut at ``depth`` rows),
+    ``accepted`` [S] (its rows; 0 for a request without rows), ``next_token`` [S] (what was chosen at its end, -1 without rows),
+    ``new_lengths`` [S] (lengths + accepted; may be ``lengths`` itself).  Trees have at most DRAFT_MAX_NODES rows; rows past
+    that are on no path."""
+    global launches
+    S = _request_ints("accept_drafts", lengths, cu_nodes)
+    for name, t in (("tokens", tokens), ("parents", parents), ("chosen", chosen), ("path", path), ("accepted", accepted),
+                    ("next_token", next_token), ("new_lengths", new_lengths)):
+        _cuda(name, t, torch.int32)
+    T = tokens.numel()
+    if parents.numel() != T or chosen.numel() != T or path.dim() != 2 or path.shape[0] != S or path.shape[1] < 1 \
+            or accepted.numel() != S or next_token.numel() != S or new_lengths.numel() != S:
+        raise KernelError(f"accept_drafts: arguments for {S} requests and {T} rows do not fit: parents {parents.numel()}, chosen "
+                          f"{chosen.numel()}, path {tuple(path.shape)}, accepted {accepted.numel()}, next_token "
+                          f"{next_token.numel()}, new_lengths {new_lengths.numel()}")
+    ld = V = slices = 0
+    part_val = part_idx = None
+    if logits is not None:
+        _cuda("logits", logits, torch.float32, contiguous=False)
+        ld = _rows("logits", logits)
+        V = logits.shape[1]
+        if logits.shape[0] != T or V < 1:
+            raise KernelError(f"accept_drafts: logits {tuple(logits.shape)} for {T} rows")
+        if T:
+            slices = library().mllm_accept_slices(T, V)
+            part_val = _scratch("accept", logits.device, 2 * T * slices).data_ptr()
+            part_idx = part_val + 4 * T * slices
+    _call("mllm_accept_drafts", None if logits is None else logits.data_ptr(), ld, T, V, slices, part_val, part_idx, chosen.data_ptr(),
+          tokens.data_ptr(), parents.data_ptr(), cu_nodes.data_ptr(), lengths.data_ptr(), S, path.data_ptr(), path.shape[1],
+          accepted.data_ptr(), next_token.data_ptr(), new_lengths.data_ptr(), _stream())
+    if slices:
+        launches += 1           # the kernel that reads the logits
+
+
+def keep_accepted(planes, block_table, lengths, path, accepted) -> None:
+    """The cache rows of an accepted path move next to the text, in place: row ``lengths[s] + path[s, k]`` of every plane and head to
+    row ``lengths[s] + k`` for k < accepted[s] (paths rise, as ``accept_drafts`` writes them; ``lengths`` are those from before it).
+    ``planes`` [..., num_pages, heads, page_size, d]: a cache group's pool, or its keys and values one after the other."""
+    _cuda("planes", planes)
+    _cuda("block_table", block_table, torch.int32, contiguous=False)
+    for name, t in (("lengths", lengths), ("path", path), ("accepted", accepted)):
+        _cuda(name, t, torch.int32)
+    S = lengths.numel()
+    bt_stride = _rows("block_table", block_table)
+    if planes.dim() < 4 or path.dim() != 2 or path.shape[0] != S or path.shape[1] < 1 or accepted.numel() != S \
+            or block_table.shape[0] != S:
+        raise KernelError(f"keep_accepted: planes {tuple(planes.shape)}, block_table {tuple(block_table.shape)}, path "
+                          f"{tuple(path.shape)}, accepted {accepted.numel()} for {S} requests")
+    P, heads, ps, d = planes.shape[-4:]
+    es = planes.element_size()
+    plane = P * heads * ps * d
+    if plane == 0:
+        return
+    _call("mllm_keep_accepted", planes.data_ptr(), plane * es, planes.numel() // plane, P, heads, ps, d * es, block_table.data_ptr(),
+          bt_stride, block_table.shape[1], lengths.data_ptr(), path.data_ptr(), path.shape[1], accepted.data_ptr(), S, _stream())
 
 
 # --------------------------------------------------------------------------- sampling
