@@ -1,0 +1,190 @@
+// What the kernels of tree attention (tree_attention.cu, tree_attention_tcgen05.cu) share: their arguments, how the work is cut,
+// which keys of a tile a row sees, and what becomes of values that are not finite.
+#pragma once
+#include "common.cuh"
+
+namespace tree {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr unsigned int NO_ROW = 0xffffffffu;
+
+struct Args {
+    const void* q; long long ldq;
+    const void* k_pages; const void* v_pages;
+    const int* block_table; int bt_stride, width;
+    const int* lengths; const int* cu_nodes; const int* ancestors; int words;
+    void* out; long long ldo;
+    float* part_o; float* part_ml;          // [2 * blocks, tile rows, dh] and [2 * blocks, tile rows, 2]
+    int S, H, Hkv, G, dh, page_size, page_shift;
+    int q_vec, out_vec;                     // queries can be read 16 bytes at a time; elements that a store may write at once
+    int tile_rows, tile_shift, max_rows;    // query rows of a tile (a power of two), and those of the largest tree's first
+    int unit_shift, blocks, max_tiles;      // keys per unit of work and blocks that share the line of units; 0: a block per pair
+    float scale_log2;
+};
+
+// ------------------------------------------------------------------------------------------------ how the work is cut
+// A pair is a tile of query rows of one (request, key/value head).  Either every pair has a block of its own (blocks == 0: the grid
+// is (head and tile, request)), or the pairs' keys are shared out evenly: each pair's keys in units of 2^unit_shift, all units of all pairs
+// in one line, in order of request, head, tile and position, and every block takes as many neighbours of that line as any other
+// (or one less), whatever the lengths.  A block's share of one pair is a segment.  Pairs that lie in one block are finished there;
+// the others leave their segments' sums in scratch, two slots a block (only its first and last segment can be parts of a pair), and
+// the join kernel adds them in order of position.  A
+// block finds its place by a scan over the requests, 32 at a time.
+struct Request { int s, first, n, len, keys, units, tiles; };
+
+__device__ __forceinline__ int keys_of(const Args& a, int len, int n) {     // those that the block table holds
+    return (int)min((long long)len + n, (long long)a.width * a.page_size);
+}
+__device__ __forceinline__ Request request_of(const Args& a, int s) {
+    Request r{s, 0, 0, 0, 0, 0, 0};
+    if (s < a.S) {
+        const int end = a.cu_nodes[s + 1], len = a.lengths[s];
+        r.first = a.cu_nodes[s];
+        r.n = end - r.first;
+        r.len = len;
+        r.keys = r.n > 0 ? keys_of(a, r.len, r.n) : 0;
+        r.units = r.keys <= 0 ? 0 : a.blocks ? ((r.keys - 1) >> a.unit_shift) + 1 : 1;
+        r.tiles = r.units ? (r.n * a.G + a.tile_rows - 1) >> a.tile_shift : 0;
+    }
+    return r;
+}
+__device__ __forceinline__ unsigned int weight_of(const Args& a, const Request& r) { return (unsigned int)r.units * r.tiles * a.Hkv; }
+
+struct Line {                               // the line of units, shared out among blocks: the first `extra` of them take per + 1
+    unsigned int units, per, extra;
+    Request mine;                           // the lane's request among the first 32
+    __device__ __forceinline__ unsigned int begin(unsigned int c) const { return c * per + min(c, extra); }
+    __device__ __forceinline__ unsigned int block_of(unsigned int u) const {
+        const unsigned int head = extra * (per + 1);
+        return u < head ? u / (per + 1) : extra + (u - head) / per;
+    }
+};
+__device__ __forceinline__ Line line_of(const Args& a) {       // all lanes of a warp together
+    Line l;
+    l.mine = request_of(a, threadIdx.x & 31);
+    unsigned int sum = weight_of(a, l.mine);
+    for (int s = 32 + (threadIdx.x & 31); s < a.S; s += 32) sum += weight_of(a, request_of(a, s));
+    l.units = __reduce_add_sync(0xffffffffu, sum);
+    l.per = l.units / a.blocks;
+    l.extra = l.units % a.blocks;
+    return l;
+}
+// The request that unit u belongs to, and the first unit of that request; all lanes together.
+__device__ __forceinline__ Request find(const Args& a, const Line& line, unsigned int u, unsigned int* base) {
+    const int lane = threadIdx.x & 31;
+    unsigned int before = 0;
+    for (int s0 = 0;; s0 += 32) {
+        const Request r = s0 == 0 ? line.mine : request_of(a, s0 + lane);
+        const unsigned int w = weight_of(a, r);
+        unsigned int incl = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned int x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        const unsigned int hit = __ballot_sync(0xffffffffu, before + incl > u);
+        if (hit || s0 + 32 >= a.S) {
+            const int l = hit ? __ffs(hit) - 1 : 31;
+            *base = before + __shfl_sync(0xffffffffu, incl - w, l);
+            return Request{s0 + l, __shfl_sync(0xffffffffu, r.first, l), __shfl_sync(0xffffffffu, r.n, l), __shfl_sync(0xffffffffu, r.len, l),
+                           __shfl_sync(0xffffffffu, r.keys, l), __shfl_sync(0xffffffffu, r.units, l), __shfl_sync(0xffffffffu, r.tiles, l)};
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+}
+struct Segment {
+    int s, first, n, len, keys;             // request, its first row in the step, its rows, its text, its keys
+    int hk, row0, rows;                     // head; the tile's first query row and the request's number of them
+    int k0, k1;                             // keys
+    int slot;                               // where its sums go; -1: it is a whole pair
+};
+// A block's segments, found by one warp for all (the same few lines of lengths and starts, read by every warp of every block, cost
+// microseconds) and left in shared memory, CAP at a time.
+struct Segments {
+    static constexpr int CAP = 8;
+    int count, more;                        // here; whether others come after them
+    unsigned int at;                        // where they begin: a unit, or a tile
+    Segment list[CAP];
+};
+__device__ __forceinline__ void first_segments(Segments* l) { l->at = 0xffffffffu; }      // one thread, before the first fill
+__device__ __forceinline__ void fill(const Args& a, Segments* l) {                        // one warp, all lanes
+    const int lane = threadIdx.x & 31;
+    unsigned int at = l->at;
+    int count = 0;
+    bool more;
+    if (!a.blocks) {
+        const Request r = request_of(a, blockIdx.y);
+        if (at == 0xffffffffu) at = blockIdx.x / a.Hkv;
+        for (; (int)at < r.tiles && count < Segments::CAP; ++count, at += a.max_tiles)     // trees larger than the host knew of go on
+            if (lane == 0)
+                l->list[count] = Segment{r.s, r.first, r.n, r.len, r.keys, (int)(blockIdx.x % a.Hkv), (int)at * a.tile_rows, r.n * a.G, 0,
+                                         r.keys, -1};
+        more = (int)at < r.tiles;
+    } else {
+        const Line line = line_of(a);
+        const unsigned int begin = line.begin(blockIdx.x), end = line.begin(blockIdx.x + 1);
+        if (at == 0xffffffffu) at = begin;
+        unsigned int base = 0;
+        Request r{};
+        bool have = false;
+        for (; at < end && count < Segments::CAP; ++count) {
+            if (!have || at - base >= weight_of(a, r)) r = find(a, line, at, &base);
+            have = true;
+            const unsigned int pair = (at - base) / r.units, unit = at - base - pair * r.units, take = min(r.units - unit, end - at);
+            const unsigned int hk = pair / r.tiles;
+            if (lane == 0)
+                l->list[count] = Segment{r.s, r.first, r.n, r.len, r.keys, (int)hk, (int)(pair - hk * r.tiles) * a.tile_rows, r.n * a.G,
+                                         (int)(unit << a.unit_shift), (int)min((long long)(unit + take) << a.unit_shift, (long long)r.keys),
+                                         take == (unsigned int)r.units ? -1 : 2 * (int)blockIdx.x + (at == begin ? 0 : 1)};
+            at += take;
+        }
+        more = at < end;
+    }
+    if (lane == 0) { l->count = count; l->more = more; l->at = at; }
+}
+
+// ------------------------------------------------------------------------------------------------ what a row sees
+// Which of the 64 keys from `key0` on a node sees: bit b for key key0 + b.  `words`: its words of bits.
+__device__ __forceinline__ unsigned long long tile_mask(const int* words, int n_words, int len, int keys, int key0, bool node) {
+    const int j0 = key0 - len;                              // place of the first key in the tree
+    auto word = [&](int w) -> unsigned long long { return w < n_words && node ? (unsigned int)words[w] : 0u; };
+    auto from = [&](int j) -> unsigned long long {          // bits j .. j + 63 of the node's words
+        const int w = j >> 5, sh = j & 31;
+        unsigned long long lo = word(w) | word(w + 1) << 32;
+        if (sh) lo = lo >> sh | word(w + 2) << (64 - sh);
+        return lo;
+    };
+    unsigned long long m = j0 >= 0 ? from(j0) : j0 <= -64 ? ~0ull : ((1ull << -j0) - 1ull) | from(0) << -j0;
+    const int left = keys - key0;                           // keys of the request from key0 on
+    if (left <= 0) return 0;
+    return left >= 64 ? m : m & ((1ull << left) - 1ull);
+}
+
+// Infinite and NaN elements of a 32-bit word (the exponent's bits all set), and the word without them.
+template <typename T> __device__ __forceinline__ bool odd_element(uint32_t w);
+template <> __device__ __forceinline__ bool odd_element<float>(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; }
+template <> __device__ __forceinline__ bool odd_element<__nv_bfloat16>(uint32_t w) {
+    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+template <typename T> __device__ __forceinline__ uint32_t without_odd(uint32_t w);
+template <> __device__ __forceinline__ uint32_t without_odd<float>(uint32_t w) { return odd_element<float>(w) ? 0u : w; }
+template <> __device__ __forceinline__ uint32_t without_odd<__nv_bfloat16>(uint32_t w) {
+    if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+    if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+    return w;
+}
+__device__ __forceinline__ float inverse_sum(float l) { return l > 0.f || l != l ? 1.f / l : 0.f; }       // nothing visible: zeros
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+inline dim3 grid_of(const Args& a) { return a.blocks ? dim3(a.blocks) : dim3(a.Hkv * a.max_tiles, a.S); }
+
+// Adds the segments of the pairs that were cut (tree_attention.cu).
+int join(const Args& a, int dtype, cudaStream_t stream);
+// bfloat16 on the fifth-generation tensor cores, tiles of 128 or 256 rows (tree_attention_tcgen05.cu).
+int tcgen05(const Args& a, long long pages, cudaStream_t stream);
+
+}  // namespace tree

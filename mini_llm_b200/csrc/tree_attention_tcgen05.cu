@@ -1,0 +1,575 @@
+// Tree attention on the fifth-generation tensor cores: bfloat16, head sizes up to 128, pages of a multiple of 8 tokens.
+// tree_attention.cu states what is computed, tree_attention.cuh how the keys are cut into blocks' segments.
+//
+// A block takes one or two tiles of 128 query rows (QT) of one key/value head and walks a segment of the request's keys in blocks
+// of 64.  NS streams know nothing of each other until the segment's end: stream x has tile x % QT and, of every NS / QT blocks, the
+// one numbered x / QT; streams of the same number read the same keys and values from shared memory.  A stream has 64 columns of
+// tensor memory for its scores and DP for its sums, and
+//  * copies of its keys and values: TMA boxes of up to 64 rows of one page, a lane each, 128-byte swizzle, zeros past the segment;
+//    the next segment's first blocks while this one's sums are read.  Heads of 64: by the stream's issuing warp, while the softmax
+//    works (with warps for the copies alone 21 or more warps would leave the softmax 80 registers, which spill); heads of 128: by a
+//    warp of its own (1,285 cycles a block out of 3,500 where the issuing warp did it);
+//  * an issuing warp: S = Q K^T (128 x 64 x 16), and O += P V with P as the MMA's tensor-memory operand and V as it lies in the
+//    pages, an MN-major operand, 64 columns at a time.  Heads of 128 have two sets of columns for scores: the next block's product
+//    runs while the softmax works on this one's;
+//  * four softmax warps, a thread per query row: 64 scores in registers, the weights as two bfloat16 terms over the scores' columns,
+//    maximum and sum in 32 bits.  m and O move only where a score exceeds m by more than 2^8.  Warps without rows only hand over.
+// At the end the streams of a tile meet in order.
+//
+// What bounds it: few rows, the cache's bytes (the MMAs are 128 rows high whatever a tree needs: 384 cycles for 64 keys of 64, whose
+// 16 KB take an SM's share of the memory 700 cycles); 256 rows of 128 columns, about equally the bytes, the MMAs (both terms of the
+// weights) and the exponentials.  Copies by TMA and not by the threads: 16-byte cp.async brought 26 bytes a cycle into an SM, and
+// that issued by warps that have the softmax to do.
+//
+// Keys that a row does not see get a weight of zero by its bits.  In blocks that reach into the tree the values' places past the
+// last key are cleared and infinite or NaN values taken out, before the product reads them; the rows that see those get them back
+// at the end.  Every wait on an mbarrier is bounded; after the limit the kernel records an error code that the host reads, lets its
+// copies land, frees its tensor memory and returns.
+#include "split_f32.cuh"
+#include "tree_attention.cuh"
+
+namespace {
+
+using namespace tc;
+using tree::Args;
+using tree::Segment;
+using tree::Segments;
+
+constexpr int BQ = 128, BKV = 64;
+constexpr float LAZY = 8.f;                          // how far (in powers of two) a score may exceed the maximum in use
+
+__device__ int g_tree_error = 0;                     // first error code seen by this kernel
+
+__host__ __device__ constexpr uint32_t make_idesc_bmn(int m, int n) { return make_idesc(m, n) | (1u << 16); }      // B MN-major
+
+__device__ __forceinline__ unsigned long long pack2(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+template <int DP, int QT>
+struct Plan {
+    static constexpr int NS = DP == 64 ? 4 : 2;                  // streams
+    static constexpr int SB = DP == 64 ? 1 : 2;                  // sets of columns for a stream's scores
+    static constexpr int KS = NS / QT;                           // streams of different keys
+    static constexpr int STAGES = 1 + 2 * QT;                        // of each of their rings of keys and values
+    static constexpr int CB = DP / 64;                           // blocks of 64 columns (128 bytes)
+    static constexpr int Q_BYTES = BQ * DP * 2;                  // of a tile
+    static constexpr int KV_BYTES = BKV * DP * 2;
+    static constexpr int SOFTMAX_WARPS = 4 * NS, ISSUE_WARP = SOFTMAX_WARPS;
+    static constexpr bool LOADER = SB > 1;                       // a warp of its own brings the keys and values
+    static constexpr int LOAD_WARP = ISSUE_WARP + NS;
+    static constexpr int THREADS = (LOAD_WARP + LOADER) * 32;    // 20 warps of 96 registers, or 11 of 168
+    static constexpr uint32_t TMEM_O = NS * SB * BKV;
+    static constexpr int Q_PIECES = QT * BQ * (DP / 8) / (SOFTMAX_WARPS * 32);         // 16-byte pieces of the queries per thread
+    static constexpr int BARRIERS = 3 * KS * STAGES + (2 * SB + 1) * NS + 1;
+    static constexpr size_t SMEM = QT * Q_BYTES + KS * STAGES * 2 * KV_BYTES + 2 * NS * BQ * 4 + BARRIERS * 8 + 16 + sizeof(Segments);
+    static_assert(TMEM_O + NS * DP <= 512, "tensor memory");
+};
+
+template <int DP, int QT>
+struct Barriers {
+    using P = Plan<DP, QT>;
+    uint64_t k_full[P::KS][P::STAGES], v_full[P::KS][P::STAGES], empty[P::KS][P::STAGES];
+    uint64_t s_full[P::NS][P::SB], p_full[P::NS][P::SB], o_full[P::NS];
+    uint64_t q_full;
+};
+
+template <int DP, int QT>
+__global__ void __launch_bounds__(Plan<DP, QT>::THREADS, 1)
+tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a,
+                              int box, int pool_rows) {
+    using P = Plan<DP, QT>;
+    using bf = __nv_bfloat16;
+    constexpr int NS = P::NS, SB = P::SB, KS = P::KS, STAGES = P::STAGES, CB = P::CB;
+    extern __shared__ __align__(1024) uint8_t base[];            // the swizzle goes by the address
+    uint8_t* sQ = base;                                           // [QT][CB][128 rows][128 bytes]
+    uint8_t* sKV = sQ + QT * P::Q_BYTES;                          // [KS][STAGES][K, V][CB][64 rows][128 bytes]
+    float* sm_m = reinterpret_cast<float*>(sKV + KS * STAGES * 2 * P::KV_BYTES);       // [NS][BQ]
+    float* sm_l = sm_m + NS * BQ;
+    Barriers<DP, QT>& bars = *reinterpret_cast<Barriers<DP, QT>*>(sm_l + NS * BQ);
+    static_assert(sizeof(Barriers<DP, QT>) == P::BARRIERS * 8, "barriers");
+    uint32_t* tmem_slot = (uint32_t*)(&bars + 1);
+    volatile int* failed = (volatile int*)(tmem_slot + 1);
+    volatile int* odd_seen = failed + 1;
+    volatile int* stop = failed + 2;
+    Segments* segments = reinterpret_cast<Segments*>(tmem_slot + 4);
+
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    if (smem_u32(base) & 1023) {
+        if (threadIdx.x == 0) { atomicCAS(&g_tree_error, 0, 11); report_to_host(1011); }
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int g = 0; g < KS; ++g)
+            for (int s = 0; s < STAGES; ++s) { mbar_init(&bars.k_full[g][s], 1); mbar_init(&bars.v_full[g][s], 1); mbar_init(&bars.empty[g][s], QT); }
+        for (int x = 0; x < NS; ++x) {
+            for (int b = 0; b < SB; ++b) { mbar_init(&bars.s_full[x][b], 1); mbar_init(&bars.p_full[x][b], 4); }
+            mbar_init(&bars.o_full[x], 1);
+        }
+        mbar_init(&bars.q_full, P::SOFTMAX_WARPS);
+        *failed = 0;
+        *odd_seen = 0;
+        tree::first_segments(segments);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x == 32) {
+        prefetch_map(&map_k);
+        prefetch_map(&map_v);
+    }
+    if (warp == P::ISSUE_WARP) tmem_alloc(tmem_slot, 512);
+    __syncwarp();
+    pdl_wait();
+    pdl_launch();
+    if (warp == 0) tree::fill(a, segments);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int G = a.G;
+    // blocks of a segment that number ks takes: from block k0 / 64 + ks on, every KS-th
+    auto steps_of = [&](const Segment& g, int ks) { const int n = (g.k1 - g.k0 + BKV - 1) / BKV - ks; return n <= 0 ? 0 : (n + KS - 1) / KS; };
+
+    // After a role has been through the list: the next part of it, if there is one and nobody gave up.  All threads.
+    auto more_segments = [&]() {
+        if (!segments->more) return false;
+        __syncthreads();
+        if (warp == 0) {
+            if (lane == 0) *stop = *failed;
+            __syncwarp();
+            if (!*stop) tree::fill(a, segments);
+        }
+        __syncthreads();
+        return !*stop;
+    };
+    // the pool row at which box `part` of the i-th block of ring ks starts; beyond the pool (zeros) where there is none
+    auto row_of = [&](const Segment& sg, int ks, int part, int i) {
+        const int kp = sg.k0 + (ks + i * KS) * BKV + part * box;
+        if (kp >= sg.k1) return pool_rows;
+        const int p = a.page_shift >= 0 ? kp >> a.page_shift : kp / a.page_size;
+        return (a.block_table[(size_t)sg.s * a.bt_stride + p] * a.Hkv + sg.hk) * a.page_size + (kp - p * a.page_size);
+    };
+    auto copy_box = [&](int ks, int s, int part, int row) {
+        uint8_t* dst = sKV + (size_t)(ks * STAGES + s) * 2 * P::KV_BYTES + (size_t)part * box * 128;
+#pragma unroll
+        for (int c = 0; c < CB; ++c) tma_load_2d(dst + c * (BKV * 128), &map_k, c * 64, row, &bars.k_full[ks][s]);
+#pragma unroll
+        for (int c = 0; c < CB; ++c) tma_load_2d(dst + P::KV_BYTES + c * (BKV * 128), &map_v, c * 64, row, &bars.v_full[ks][s]);
+    };
+    const int boxes = BKV / box;
+
+    if (P::LOADER && warp == P::LOAD_WARP) {
+        // ---------------------------------------------------------------- keys and values: eight lanes a ring, lane p of them box p
+        const int ks = lane >> 3, part = lane & 7;
+        const bool mine = ks < KS && part < boxes;
+        int it = 0;                                               // blocks of this lane's ring so far, of all segments
+        bool ok = true;
+        do {
+            for (int n = 0; ok && n < segments->count; ++n) {
+                const Segment& sg = segments->list[n];
+                const int steps = ks < KS ? steps_of(sg, ks) : 0, most = steps_of(sg, 0);
+                int row = mine ? row_of(sg, ks, part, 0) : 0;
+                for (int i = 0; i < most; ++i) {
+                    const bool on = i < steps;
+                    const int s = it % STAGES;
+                    const int next = mine ? row_of(sg, ks, part, i + 1) : 0;
+                    ok = !on || it < STAGES || mbar_wait(&bars.empty[ks][s], ((it / STAGES) - 1) & 1);
+                    if (!ok) *failed = 1;
+                    ok = __all_sync(0xffffffffu, ok && !*failed);
+                    if (!ok) break;
+                    if (on && part == 0) {
+                        mbar_expect_tx(&bars.k_full[ks][s], P::KV_BYTES);
+                        mbar_expect_tx(&bars.v_full[ks][s], P::KV_BYTES);
+                    }
+                    __syncwarp();
+                    if (on && mine) copy_box(ks, s, part, row);
+                    row = next;
+                    it += on;
+                }
+            }
+        } while (more_segments());
+    } else if (warp >= P::ISSUE_WARP) {
+        // ---------------------------------------------------------------- a stream's MMAs (and copies)
+        const int x = warp - P::ISSUE_WARP, qt = x % QT, ks = x / QT;
+        constexpr uint32_t idesc_s = make_idesc(BQ, BKV), idesc_o = make_idesc_bmn(BQ, 64);
+        const uint64_t q_desc = make_smem_desc(smem_u32(sQ + qt * P::Q_BYTES)),
+                       kv_desc = make_smem_desc(smem_u32(sKV + (size_t)ks * STAGES * 2 * P::KV_BYTES));
+        const uint32_t t_s = tmem + (uint32_t)(x * SB * BKV), t_o = tmem + P::TMEM_O + (uint32_t)(x * DP);
+        auto all_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity) && !*failed); };
+        int it = 0, done = 0, turn = 0, loaded = 0;           // blocks, commits to o_full, segments so far; blocks asked for
+        bool ok = true;
+        auto give_up = [&](int code) { if (!*failed) *failed = code; return false; };
+        // the scores of block n of the stream
+        auto scores = [&](int n) {
+            const int s = n % STAGES, b = n % SB;
+            if (!all_wait(&bars.k_full[ks][s], (n / STAGES) & 1)) return give_up(4);
+            tc_fence_after();
+            const uint64_t k_desc = kv_desc + (uint64_t)(s * (2 * P::KV_BYTES >> 4));
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k)
+                umma_f16_warp(t_s + (uint32_t)(b * BKV), q_desc + (uint64_t)((k >> 2) * (BQ * 128 >> 4) + 2 * (k & 3)),
+                              k_desc + (uint64_t)((k >> 2) * (BKV * 128 >> 4) + 2 * (k & 3)), idesc_s, k != 0);
+            umma_commit_warp(&bars.s_full[x][b]);
+            return true;
+        };
+        do {
+        for (int n = 0; ok && n < segments->count; ++n, ++turn) {
+            const Segment& sg = segments->list[n];
+            const int steps = steps_of(sg, ks);
+            int asked = 0, row = 0;                           // the next block to ask for, and where this lane's box of it starts
+            auto load = [&]() {                               // once the MMAs have read what lies in its place
+                if (P::LOADER || qt != 0 || asked >= steps) return true;
+                const int s = loaded % STAGES;
+                if (loaded >= STAGES && !all_wait(&bars.empty[ks][s], ((loaded / STAGES) - 1) & 1)) return give_up(1);
+                if (lane == 0) {
+                    mbar_expect_tx(&bars.k_full[ks][s], P::KV_BYTES);
+                    mbar_expect_tx(&bars.v_full[ks][s], P::KV_BYTES);
+                }
+                __syncwarp();
+                if (lane < boxes) copy_box(ks, s, lane, row);
+                ++loaded;
+                ++asked;
+                if (lane < boxes) row = row_of(sg, ks, lane, asked);
+                return true;
+            };
+            if (!P::LOADER && lane < boxes) row = row_of(sg, ks, lane, 0);
+            for (int i = 0; i < STAGES && ok; ++i) ok = load();
+            if (!ok) break;
+            ok = all_wait(&bars.q_full, turn & 1);                // the queries are in, and the last segment's sums have been read
+            if (!ok) { give_up(2); break; }
+            if (steps == 0) { umma_commit_warp(&bars.o_full[x]); ++done; }          // nothing to do, but the softmax warps wait to hear it
+            else if (SB > 1) ok = scores(it);
+            for (int i = 0; i < steps && ok; ++i, ++it, ++done) {
+                // a set of columns is free for scores once the product that read its last weights is complete
+                if (i > 0 && (SB == 1 || i + 1 < steps) && !all_wait(&bars.o_full[x], (done - 1) & 1)) { ok = give_up(3); break; }
+                if (SB == 1 || i + 1 < steps) ok = scores(it + SB - 1);
+                if (ok && i > 0) ok = load();
+                if (!ok) break;
+                const int s = it % STAGES, b = it % SB;
+                if (!all_wait(&bars.v_full[ks][s], (it / STAGES) & 1)) { ok = give_up(5); break; }
+                if (!all_wait(&bars.p_full[x][b], (it / SB) & 1)) { ok = give_up(6); break; }
+                tc_fence_after();
+                const uint64_t v_desc = kv_desc + (uint64_t)(s * (2 * P::KV_BYTES >> 4)) + (uint64_t)(P::KV_BYTES >> 4);
+#pragma unroll
+                for (int c = 0; c < CB; ++c)
+#pragma unroll
+                    for (int term = 0; term < 2; ++term)          // hi, then lo
+#pragma unroll
+                        for (int kk = 0; kk < BKV / 16; ++kk)
+                            umma_f16_ts_warp(t_o + (uint32_t)(c * 64), t_s + (uint32_t)(b * BKV + term * (BKV / 2) + kk * 8),
+                                             v_desc + (uint64_t)(c * (BKV * 128 >> 4) + kk * (2048 >> 4)), idesc_o, (i | term | kk) != 0);
+                umma_commit_warp(&bars.o_full[x]);
+                umma_commit_warp(&bars.empty[ks][s]);
+            }
+        }
+        } while (more_segments());
+    } else {
+        // ---------------------------------------------------------------- softmax: one query row per thread
+        const int x = warp >> 2, qt = x % QT, ks = x / QT;
+        const int q4 = warp & 3;                              // the quarter of the tensor-memory lanes this warp may read
+        const int r = q4 * 32 + lane;                         // row of the tile
+        const uint32_t t_lane = (uint32_t)(q4 * 32) << 16;
+        const uint32_t t_s0 = tmem + (uint32_t)(x * SB * BKV) + t_lane, t_o = tmem + P::TMEM_O + (uint32_t)(x * DP) + t_lane;
+        const float sl2 = a.scale_log2;
+        const unsigned long long sl2_2 = pack2(sl2, sl2);
+        int it = 0, done = 0;                                 // blocks, commits to o_full so far
+        bool alive = true;
+        do {
+        for (int n = 0; alive && n < segments->count; ++n) {
+            const Segment& sg = segments->list[n];
+            const int rows = sg.rows - sg.row0;               // query rows of the block's tiles
+            // ---- the queries, 16-byte pieces, up to eight of a thread's in flight; rows past the end are never looked at
+            constexpr int BATCH = P::Q_PIECES < 8 ? P::Q_PIECES : 8;
+#pragma unroll 1
+            for (int i0 = 0; i0 < P::Q_PIECES; i0 += BATCH) {
+                uint4 v[BATCH];
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const int e = threadIdx.x + (i0 + i) * (P::SOFTMAX_WARPS * 32), row = e / (DP / 8), c = e % (DP / 8);
+                    v[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (row >= rows || c * 8 >= a.dh) continue;
+                    const bf* src = static_cast<const bf*>(a.q) + (size_t)(sg.first + (sg.row0 + row) / G) * a.ldq +
+                                    (size_t)(sg.hk * G + (sg.row0 + row) % G) * a.dh + c * 8;
+                    if (a.q_vec) {
+                        v[i] = *reinterpret_cast<const uint4*>(src);
+                    } else {
+                        const unsigned short* w = reinterpret_cast<const unsigned short*>(src);
+                        v[i] = make_uint4(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16, w[4] | (uint32_t)w[5] << 16, w[6] | (uint32_t)w[7] << 16);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const int e = threadIdx.x + (i0 + i) * (P::SOFTMAX_WARPS * 32), row = e / (DP / 8), c = e % (DP / 8);
+                    if (row < rows)
+                        *reinterpret_cast<uint4*>(sQ + (row / BQ) * P::Q_BYTES + (c >> 3) * (BQ * 128) + (row % BQ) * 128 + ((c ^ row) & 7) * 16) = v[i];
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.q_full);
+
+            const int steps = steps_of(sg, ks);
+            const int tile_row = qt * BQ + r;                 // row among the block's tiles
+            const bool active = qt * BQ + q4 * 32 < rows;
+            const int node = tile_row < rows ? (sg.row0 + tile_row) / G : 0;
+            const int* words = a.ancestors + (size_t)(sg.first + node) * a.words;
+            const int tail_from = min(sg.len, sg.keys);   // from here on rows do not all see what is there
+            float m_run = -INFINITY, l_run = 0.f;
+            for (int i = 0; i < steps; ++i, ++it) {
+                const int key0 = sg.k0 + (ks + i * KS) * BKV;
+                const bool tail = key0 + BKV > tail_from;
+                unsigned long long seen = ~0ull;
+                if (tail) {
+                    if (active) seen = tree::tile_mask(words, a.words, sg.len, sg.keys, key0, tile_row < rows);
+                    // values past the last key and those that are not finite: out, before the product reads them
+                    const int s = it % STAGES;
+                    bool got = mbar_wait(&bars.v_full[ks][s], (it / STAGES) & 1);
+                    if (!got) *failed = 9;
+                    uint8_t* tv = sKV + (size_t)(ks * STAGES + s) * 2 * P::KV_BYTES + P::KV_BYTES;
+                    for (int e = r; got && e < BKV * DP / 8; e += BQ) {
+                        const int kp = key0 + (e / 8) % BKV;
+                        if (kp < tail_from) continue;
+                        uint4* w = reinterpret_cast<uint4*>(tv + e * 16);
+                        uint4 v = *w;
+                        if (kp >= sg.keys) {
+                            *w = make_uint4(0u, 0u, 0u, 0u);
+                        } else if (tree::odd_element<bf>(v.x) || tree::odd_element<bf>(v.y) || tree::odd_element<bf>(v.z) || tree::odd_element<bf>(v.w)) {
+                            *w = make_uint4(tree::without_odd<bf>(v.x), tree::without_odd<bf>(v.y), tree::without_odd<bf>(v.z), tree::without_odd<bf>(v.w));
+                            *odd_seen = 1;
+                        }
+                    }
+                    fence_async_smem();
+                }
+                const int b = it % SB;
+                const uint32_t t_s = t_s0 + (uint32_t)(b * BKV);
+                bool got = mbar_wait(&bars.s_full[x][b], (it / SB) & 1);
+                if (!got) *failed = 7;
+                alive = __all_sync(0xffffffffu, got && !*failed);
+                if (!alive) break;
+                if (active) {
+                    tc_fence_after();
+                    uint32_t v[2][32];
+                    tmem_ld32_issue(t_s, v[0]);
+                    tmem_ld32_issue(t_s + 32, v[1]);
+                    tmem_ld_wait();
+                    if (tail) {
+#pragma unroll
+                        for (int e = 0; e < 64; ++e)
+                            if (!(seen >> e & 1)) v[e >> 5][e & 31] = __float_as_uint(-INFINITY);
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int e = 0; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(v[e >> 5][e & 31]));
+                    // the maximum comes off a score before the scale goes on: no score of any size ends above it by a rounding
+                    const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    const bool moves = (mb - m_run) * sl2 > LAZY;     // (from -inf on: any visible key)
+                    if (__any_sync(0xffffffffu, moves)) {
+                        const float alpha = moves ? tree::fast_exp2((m_run - mb) * sl2) : 1.f;
+                        if (moves) m_run = mb;
+                        l_run *= alpha;
+                        if (i > 0) {
+                            if (SB > 1) {                             // the last block's product may still be adding to the sums
+                                bool there = mbar_wait(&bars.o_full[x], (done + i - 1) & 1);
+                                if (!there) *failed = 10;
+                                tc_fence_after();
+                            }
+#pragma unroll
+                            for (int c = 0; c < DP; c += 16) {
+                                uint32_t w[16];
+                                tmem_ld16_issue(t_o + c, w);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * alpha);
+                                tmem_st8(t_o + c, make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7]));
+                                tmem_st8(t_o + c + 8, make_uint4(w[8], w[9], w[10], w[11]), make_uint4(w[12], w[13], w[14], w[15]));
+                            }
+                        }
+                    }
+                    const float muse = m_run == -INFINITY ? 0.f : m_run;
+                    const unsigned long long neg = pack2(-muse, -muse);
+                    unsigned long long rs[2] = {0ull, 0ull};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {                     // 16 keys: 8 columns of each term
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int k = c * 16 + 2 * e;
+                            const float2 t = unpack2(mul2(add2(pack2(__uint_as_float(v[k >> 5][k & 31]), __uint_as_float(v[k >> 5][(k & 31) + 1])), neg), sl2_2));
+                            const unsigned long long p = pack2(tree::fast_exp2(t.x), tree::fast_exp2(t.y));
+                            rs[e & 1] = add2(rs[e & 1], p);
+                            const float2 pf = unpack2(p);
+                            hi[e] = bf16x2_rn(pf.x, pf.y);
+                            const float2 left = unpack2(add2(p, pack2(-__uint_as_float(hi[e] << 16), -__uint_as_float(hi[e] & 0xffff0000u))));
+                            lo[e] = bf16x2_rn(left.x, left.y);
+                        }
+                        tmem_st8(t_s + c * 8, make_uint4(hi[0], hi[1], hi[2], hi[3]), make_uint4(hi[4], hi[5], hi[6], hi[7]));
+                        tmem_st8(t_s + 32 + c * 8, make_uint4(lo[0], lo[1], lo[2], lo[3]), make_uint4(lo[4], lo[5], lo[6], lo[7]));
+                    }
+                    const float2 sum = unpack2(add2(rs[0], rs[1]));
+                    l_run += sum.x + sum.y;
+                    tmem_st_wait();
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.p_full[x][b]);
+            }
+            done += max(steps, 1);
+            if (alive) {
+                bool got = mbar_wait(&bars.o_full[x], (done - 1) & 1);
+                if (!got) *failed = 8;
+                alive = __all_sync(0xffffffffu, got && !*failed);
+            }
+            // ---- the streams of a row meet, in order; thread (ks, r) writes its share of the columns
+            sm_m[x * BQ + r] = m_run;
+            sm_l[x * BQ + r] = l_run;
+            if (KS > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + qt * 4 + q4), "n"(KS * 32) : "memory");
+            else __syncwarp();
+            if (alive && active) {
+                tc_fence_after();
+                float m = -INFINITY, l = 0.f;
+#pragma unroll
+                for (int y = 0; y < KS; ++y) m = fmaxf(m, sm_m[(y * QT + qt) * BQ + r]);
+                float f[KS];
+#pragma unroll
+                for (int y = 0; y < KS; ++y) {
+                    const float my = sm_m[(y * QT + qt) * BQ + r];
+                    f[y] = my == -INFINITY ? 0.f : tree::fast_exp2((my - m) * sl2);
+                    l = fmaf(f[y], sm_l[(y * QT + qt) * BQ + r], l);
+                }
+                const int q = sg.row0 + tile_row;
+                const float inv = tree::inverse_sum(l);
+                const size_t pr = (size_t)max(sg.slot, 0) * a.tile_rows + tile_row;
+                if (sg.slot >= 0 && tile_row < rows && ks == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = make_float2(m, l);
+                bf* orow = static_cast<bf*>(a.out) + (size_t)(sg.first + node) * a.ldo + (size_t)(sg.hk * G + q % G) * a.dh;
+#pragma unroll 1
+                for (int c0 = ks * (DP / KS); c0 < (ks + 1) * (DP / KS) && c0 < a.dh; c0 += 16) {
+                    float o[16];
+                    uint32_t w[KS][16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = 0.f;
+#pragma unroll
+                    for (int y = 0; y < KS; ++y)
+                        tmem_ld16_issue(tmem + P::TMEM_O + t_lane + (uint32_t)((y * QT + qt) * DP + c0), w[y]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int y = 0; y < KS; ++y) {
+                        if (steps_of(sg, y) == 0) continue;           // uniform: the stream's columns were not written
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = fmaf(f[y], __uint_as_float(w[y][e]), o[e]);
+                    }
+                    if (tile_row >= rows) continue;
+                    if (*odd_seen) {                                  // values that are not finite, to the rows that see them
+                        const int* bt = a.block_table + (size_t)sg.s * a.bt_stride;
+                        for (int kp = max(sg.k0, tail_from); kp < sg.k1; ++kp) {
+                            const int j = kp - sg.len;
+                            if (j < 0 || j >= 32 * a.words || !((unsigned int)words[j >> 5] >> (j & 31) & 1)) continue;
+                            const int p = kp / a.page_size;
+                            const bf* vrow = static_cast<const bf*>(a.v_pages) + (((size_t)bt[p] * a.Hkv + sg.hk) * a.page_size + kp % a.page_size) * a.dh + c0;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const float v = __bfloat162float(vrow[e]);
+                                if (!(fabsf(v) < INFINITY)) o[e] += v;
+                            }
+                        }
+                    }
+                    if (sg.slot >= 0) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            *reinterpret_cast<float4*>(a.part_o + pr * a.dh + c0 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    } else {
+                        uint32_t h[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) h[e] = bf16x2_rn(o[2 * e] * inv, o[2 * e + 1] * inv);
+                        if (a.out_vec >= 8) {
+                            *reinterpret_cast<uint4*>(orow + c0) = make_uint4(h[0], h[1], h[2], h[3]);
+                            *reinterpret_cast<uint4*>(orow + c0 + 8) = make_uint4(h[4], h[5], h[6], h[7]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) orow[c0 + e] = __ushort_as_bfloat16((unsigned short)(h[e >> 1] >> (16 * (e & 1))));
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            // all warps are done with the queries, maxima and sums before the next segment's are written
+            asm volatile("bar.sync 15, %0;" ::"n"(P::SOFTMAX_WARPS * 32) : "memory");
+            if (threadIdx.x == 0) {
+                *odd_seen = 0;
+                *stop = *failed;                              // one reading for all: they go on together or not at all
+            }
+            asm volatile("bar.sync 15, %0;" ::"n"(P::SOFTMAX_WARPS * 32) : "memory");
+            alive = !*stop;
+        }
+        } while (more_segments());
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (*failed) {
+        if (threadIdx.x == 0) { atomicCAS(&g_tree_error, 0, *failed); report_to_host(1000 + *failed); }
+        for (int i = 0; i < 2000; ++i) __nanosleep(100);          // copies and MMAs already issued may still be running
+        __syncthreads();
+    }
+    if (warp == P::ISSUE_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int DP, int QT>
+int launch(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, int box, int pool_rows, cudaStream_t stream) {
+    using P = Plan<DP, QT>;
+    static_assert(P::SMEM <= 232448, "shared memory of a block");
+    auto kern = tree_attention_tcgen05_kernel<DP, QT>;
+    static bool set = false;
+    if (!set) {
+        MLLM_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::SMEM));
+        set = true;
+    }
+    MLLM_CUDA(mllm_launch(kern, tree::grid_of(a), dim3(P::THREADS), P::SMEM, stream, true, mk, mv, a, box, pool_rows));
+    return a.blocks ? tree::join(a, MLLM_BF16, stream) : 0;
+}
+
+}  // namespace
+
+// The pinned host word that this file's kernels write when they give up on a wait.
+MLLM_EXPORT int mllm_tree_attention_bind_error(int* word) { return bind_host_error(word); }
+
+// The first error recorded by the kernel since the last call (0 = none); resets it.
+MLLM_EXPORT int mllm_tree_attention_error(int* code) {
+    int zero = 0;
+    MLLM_CUDA(cudaMemcpyFromSymbol(code, g_tree_error, sizeof(int)));
+    if (*code) MLLM_CUDA(cudaMemcpyToSymbol(g_tree_error, &zero, sizeof(int)));
+    return 0;
+}
+
+int tree::tcgen05(const Args& a, long long pages, cudaStream_t stream) {
+    const long long rows = pages * a.Hkv * a.page_size;
+    int box = 64;
+    while (a.page_size % box) box >>= 1;
+    if (a.dh > 128 || box < 8 || rows + 64 > 0x7fffffffLL || (a.tile_rows != BQ && a.tile_rows != 2 * BQ))
+        return mllm_fail(1, "tree_attention: the tcgen05 kernel takes heads of up to 128, pages of a multiple of 8 tokens and "
+                            "tiles of 128 or 256 rows, not %d, %d, %d", a.dh, a.page_size, a.tile_rows);
+    CUtensorMap mk, mv;
+    int rc = get_map(a.k_pages, a.dh, (int)rows, a.dh, 64, box, MAP_BF16_SW128, &mk);
+    if (rc) return rc;
+    rc = get_map(a.v_pages, a.dh, (int)rows, a.dh, 64, box, MAP_BF16_SW128, &mv);
+    if (rc) return rc;
+    if (a.dh <= 64) return a.tile_rows == BQ ? launch<64, 1>(a, mk, mv, box, (int)rows, stream) : launch<64, 2>(a, mk, mv, box, (int)rows, stream);
+    return a.tile_rows == BQ ? launch<128, 1>(a, mk, mv, box, (int)rows, stream) : launch<128, 2>(a, mk, mv, box, (int)rows, stream);
+}

@@ -120,9 +120,12 @@ def _signatures(lib):
         "mllm_draft_max_nodes": [],
         "mllm_draft_tables": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
                               c_void_p, c_void_p, c_void_p, c_int, c_void_p],
+        "mllm_tree_attention_bind_error": [c_void_p],
+        "mllm_tree_attention_error": [c_void_p],
+        "mllm_tree_attention_per_sm": [c_int, c_int, c_int],
         "mllm_tree_attention": [c_void_p, c_ll, c_void_p, c_void_p, c_ll, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int,
-                                c_void_p, c_ll, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
-                                c_int, c_int, c_void_p],
+                                c_void_p, c_ll, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
+                                c_int, c_int, c_int, c_void_p],
         "mllm_accept_slices": [c_int, c_int],
         "mllm_accept_drafts": [c_void_p, c_ll, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
@@ -257,7 +260,7 @@ def _bind_error_word(lib) -> None:
     for name in ("mllm_tcgen05_bind_error", "mllm_attention_tcgen05_bind_error", "mllm_attention_decode_bind_error",
                  "mllm_linear_stream_f32_bind_error", "mllm_linear_split_f32_bind_error",
                  "mllm_linear_cluster_bind_error", "mllm_attention_split_f32_bind_error", "mllm_linear_batch_f32_bind_error",
-                 "mllm_moe_split_f32_bind_error"):
+                 "mllm_moe_split_f32_bind_error", "mllm_tree_attention_bind_error"):
         if getattr(lib, name)(word.data_ptr()) != 0:
             raise KernelError(lib.mllm_last_error().decode(errors="replace"))
     _error_word = word
@@ -266,7 +269,8 @@ def _bind_error_word(lib) -> None:
 _WHO = {1: "the tcgen05 product", 2: "the tcgen05 attention", 3: "the decode attention",
         4: "the float32 weight-streaming product", 5: "the float32 product of many rows",
         6: "the product of a decode batch", 7: "the float32 prefill attention",
-        8: "the float32 product of a decode batch", 9: "the float32 product of routed experts"}
+        8: "the float32 product of a decode batch", 9: "the float32 product of routed experts",
+        10: "the tree attention"}
 
 
 def raise_if_kernel_gave_up() -> None:
@@ -390,6 +394,11 @@ def check_device_errors() -> None:
     if code.value:
         raise KernelError(f"the float32 product of routed experts gave up waiting: code {code.value} "
                           "(1, 5 the cutting warps, 2-3 the MMA issuer, 4 the epilogue, 6 the TMA producer)")
+    if lib.mllm_tree_attention_error(ctypes.byref(code)) != 0:
+        raise KernelError(lib.mllm_last_error().decode(errors="replace"))
+    if code.value:
+        raise KernelError(f"the tree attention gave up waiting: code {code.value} "
+                          "(1-6 the issuing warps, 7-10 the softmax warps, 11 shared memory is not aligned)")
 
 
 class _Scope(threading.local):
@@ -422,7 +431,7 @@ class stream_scope:
 
 def _stream() -> int:
     handle = _scope.handle
-    return handle if handle is not None else torch.cuda.current_stream().cuda_stream
+    return handle if handle is not None else torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _with_company(company) -> None:
@@ -990,7 +999,9 @@ def _scratch(name: str, device, floats: int) -> torch.Tensor:
     the call's stream afterwards."""
     if _scope.workspace is not None:
         return _scope.workspace.flat(name, floats)
-    with torch.cuda.stream(_scope.stream):          # (None: the current stream)
+    if _scope.stream is None:                       # the current stream
+        return torch.empty(int(floats), dtype=torch.float32, device=device)
+    with torch.cuda.stream(_scope.stream):
         return torch.empty(int(floats), dtype=torch.float32, device=device)
 
 
@@ -2355,7 +2366,6 @@ def _attend(impl, q, ldq, k_pages, v_pages, block_table, bt_stride, ctx, out, ld
 # that it hangs on (parents: an earlier row; -1: on the text itself).  Lengths, trees and results are int32 tensors on the device, so
 # that a step can follow the one before it without the host knowing how many tokens that one kept.  A request may bring no row.
 DRAFT_MAX_NODES = 256
-TREE_ATTN_TARGET_BLOCKS = 592      # blocks that a tree attention is cut into where its keys allow: four per SM
 
 
 def _request_ints(who: str, lengths, cu_nodes) -> int:
@@ -2406,15 +2416,27 @@ def draft_tables(lengths, cu_nodes, parents, pages, cu_pages, page_size: int, *,
           None if ancestors is None else ancestors.data_ptr(), words, _stream())
 
 
+TREE_UNIT = 64               # keys of a unit of work of a tree attention that is cut along its keys
+TREE_JOIN_KEYS = 512         # what joining the parts costs, in keys that a block could walk instead
+
+
 @functools.lru_cache(maxsize=1024)
-def tree_plan(float32: bool, S: int, num_heads: int, num_kv_heads: int, max_nodes: int, max_length: int):
-    """(query rows per block, blocks that share a key/value head's rows, spans of a request's keys) of a tree attention: the
-    smallest tile that holds a tree's rows, and as many spans as it takes to fill the GPU, none under 64 keys."""
+def tree_plan(float32: bool, S: int, num_heads: int, num_kv_heads: int, head_dim: int, max_nodes: int, max_length: int, tcgen05: bool,
+              sms: int):
+    """How a tree attention is cut: (query rows of a tile, those of the largest tree, blocks that share the keys evenly (0: one for
+    every pair of tile and key/value head), whether a pair's block is a wide one).  ``tcgen05``: the kernel on tensor memory takes
+    these heads and pages."""
     rows = max(1, max_nodes * (num_heads // num_kv_heads))
-    tile = next((t for t in ((4, 8, 16) if float32 else (16, 32)) if rows <= t), 64)
-    tiles = min(-(-rows // tile), 65535 // num_kv_heads)
-    most = -(-(max_length + max_nodes) // 64)
-    return tile, tiles, max(1, min(-(-TREE_ATTN_TARGET_BLOCKS // (S * num_kv_heads * tiles)), most, 64))
+    if tcgen05:
+        tile = 128 if rows <= 128 else 256
+    else:
+        tile = next((t for t in ((4, 8, 16, 32) if float32 else (16, 32)) if rows <= t), 64)
+    tiles = -(-rows // tile)
+    pairs, places = S * num_kv_heads * tiles, sms * library().mllm_tree_attention_per_sm(head_dim, tile, F32 if float32 else BF16)
+    keys = max_length + max_nodes
+    if -(-pairs // places) * keys <= pairs * keys // places + TREE_JOIN_KEYS:
+        return tile, rows, 0, pairs <= sms
+    return tile, rows, places, False
 
 
 def tree_attention(q, k_pages, v_pages, block_table, lengths, cu_nodes, ancestors, out, *, num_heads, num_kv_heads, head_dim, scale,
@@ -2451,19 +2473,21 @@ def tree_attention(q, k_pages, v_pages, block_table, lengths, cu_nodes, ancestor
     if T == 0 or S == 0:
         return
     width, words = block_table.shape[1], ancestors.shape[1]
-    tile, tiles, splits = tree_plan(dt == F32, S, num_heads, num_kv_heads, min(T, 32 * words if max_nodes is None else int(max_nodes)),
-                                    width * ps if max_length is None else min(int(max_length), width * ps))
+    tile, rows, blocks, wide = tree_plan(
+        dt == F32, S, num_heads, num_kv_heads, head_dim, min(T, 32 * words if max_nodes is None else int(max_nodes)),
+        width * ps if max_length is None else min(int(max_length), width * ps),
+        dt == BF16 and use_tcgen05_attention and head_dim <= 128 and ps % 8 == 0, sm_count())
     part_o = part_ml = None
-    if splits > 1:
-        part = _scratch("tree_attn", q.device, splits * T * num_heads * (head_dim + 2))
-        part_o = part.data_ptr()
-        part_ml = part_o + 4 * splits * T * num_heads * head_dim
+    if blocks:
+        parts = 2 * blocks * tile
+        part_o = _scratch("tree_attn", q.device, parts * (head_dim + 2)).data_ptr()
+        part_ml = part_o + 4 * parts * head_dim
     attention_launches["tree"] = attention_launches.get("tree", 0) + 1
     _call("mllm_tree_attention", q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), P, block_table.data_ptr(), bt_stride, width,
-          lengths.data_ptr(), cu_nodes.data_ptr(), ancestors.data_ptr(), words, out.data_ptr(), ldo, part_o, part_ml, T, S, num_heads,
-          num_kv_heads, head_dim, ps, float(scale), tile, tiles, splits, dt, _stream())
-    if splits > 1:
-        launches += 1           # the kernel in which the spans meet
+          lengths.data_ptr(), cu_nodes.data_ptr(), ancestors.data_ptr(), words, out.data_ptr(), ldo, part_o, part_ml, S, num_heads,
+          num_kv_heads, head_dim, ps, float(scale), tile, rows, TREE_UNIT, blocks, wide, dt, _stream())
+    if blocks:
+        launches += 1           # the kernel in which the parts meet
 
 
 def accept_drafts(tokens, parents, cu_nodes, lengths, *, chosen, path, accepted, next_token, new_lengths, logits=None) -> None:
