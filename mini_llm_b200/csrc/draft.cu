@@ -254,68 +254,76 @@ keep_accepted_kernel(U* planes, long long plane_stride, int n_planes, int pages,
 
 MLLM_EXPORT int mllm_draft_max_nodes() { return MAX_NODES; }
 
-// parents may be null (every row follows the one before it), ancestors then too.
-MLLM_EXPORT int mllm_draft_tables(const int* lengths, const int* cu_nodes, const int* parents, const int* pages, const int* cu_pages,
-                                  int S, int page_size, int* block_table, int width, int* slots, int* positions, int* token_seq,
-                                  int* ctx_len, int* ancestors, int words, cudaStream_t stream) {
-    if (S <= 0) return 0;
-    if (page_size <= 0 || width <= 0) return mllm_fail(1, "draft_tables: pages of %d tokens, a table of %d columns", page_size, width);
-    if ((parents && !ancestors) || (ancestors && (words <= 0 || words > MAX_NODES / 32)))
-        return mllm_fail(1, "draft_tables: a tree needs 1 to %d words of bits per row, got %d", MAX_NODES / 32, ancestors ? words : 0);
+// The three entry points take their arguments packed in one block of 64-bit fields: a call from Python converts every argument of its
+// own, 0.12 us each, which for 20 to 30 of them is more than the launch.
+struct DraftTablesArgs {
+    const int *lengths, *cu_nodes, *parents, *pages, *cu_pages;      // parents may be null (every row follows the one before it),
+    int *block_table, *slots, *positions, *token_seq, *ctx_len, *ancestors;      // ancestors then too
+    long long S, page_size, width, words;
+};
+MLLM_EXPORT int mllm_draft_tables(const DraftTablesArgs* a, cudaStream_t stream) {
+    if (a->S <= 0) return 0;
+    if (a->page_size <= 0 || a->width <= 0)
+        return mllm_fail(1, "draft_tables: pages of %lld tokens, a table of %lld columns", a->page_size, a->width);
+    if ((a->parents && !a->ancestors) || (a->ancestors && (a->words <= 0 || a->words > MAX_NODES / 32)))
+        return mllm_fail(1, "draft_tables: a tree needs 1 to %d words of bits per row, got %lld", MAX_NODES / 32, a->ancestors ? a->words : 0);
     // a block writes up to 1,024 columns of the table
-    const int slices = (width + 4 * TABLE_THREADS - 1) / (4 * TABLE_THREADS);
-    if (slices > 65535) return mllm_fail(1, "draft_tables: a table of %d columns is more than one launch takes", width);
-    MLLM_CUDA(mllm_launch(draft_tables_kernel, dim3(S, slices), dim3(TABLE_THREADS), 0, stream, true, lengths, cu_nodes, parents,
-                          pages, cu_pages, page_size, block_table, width, slots, positions, token_seq, ctx_len, ancestors, words));
+    const long long slices = (a->width + 4 * TABLE_THREADS - 1) / (4 * TABLE_THREADS);
+    if (slices > 65535) return mllm_fail(1, "draft_tables: a table of %lld columns is more than one launch takes", a->width);
+    MLLM_CUDA(mllm_launch(draft_tables_kernel, dim3((unsigned)a->S, (unsigned)slices), dim3(TABLE_THREADS), 0, stream, true, a->lengths,
+                          a->cu_nodes, a->parents, a->pages, a->cu_pages, (int)a->page_size, a->block_table, (int)a->width, a->slots,
+                          a->positions, a->token_seq, a->ctx_len, a->ancestors, (int)a->words));
     return 0;
 }
 
-// Slices into which a row of V logits is cut: enough blocks for every SM, no slice under 2,048 logits.
-MLLM_EXPORT int mllm_accept_slices(int rows, int V) {
-    const int want = rows > 0 ? (4736 + rows - 1) / rows : 1;          // 32 blocks per SM
-    const int most = (V + 2047) / 2048;
-    return want < most ? (want < 1 ? 1 : want) : (most < 1 ? 1 : most);
-}
-
-// logits null: `chosen` is read instead of written.  part_val, part_idx: rows x slices of scratch.
-MLLM_EXPORT int mllm_accept_drafts(const float* logits, long long ld, int T, int V, int slices, float* part_val, int* part_idx,
-                                   int* chosen, const int* tokens, const int* parents, const int* cu_nodes, const int* lengths,
-                                   int S, int* path, int depth, int* accepted, int* next_token, int* new_lengths,
-                                   cudaStream_t stream) {
-    if (S <= 0) return 0;
-    if (depth <= 0) return mllm_fail(1, "accept_drafts: paths of %d rows", depth);
-    if (logits && T > 0) {
-        if (V <= 0 || slices <= 0 || (long long)T * slices > 0x7fffffffLL)
-            return mllm_fail(1, "accept_drafts: vocabulary %d, %d rows in %d slices", V, T, slices);
-        MLLM_CUDA(mllm_launch(accept_scan_kernel, dim3(T * slices), dim3(SCAN_THREADS), 0, stream, true, logits, ld, V, slices,
-                              part_val, part_idx));
+// logits null: `chosen` is read instead of written.  part_val, part_idx: T x slices of scratch.
+struct AcceptArgs {
+    const float* logits;
+    float* part_val;
+    int *part_idx, *chosen;
+    const int *tokens, *parents, *cu_nodes, *lengths;
+    int *path, *accepted, *next_token, *new_lengths;
+    long long ld, T, V, slices, S, depth;
+};
+MLLM_EXPORT int mllm_accept_drafts(const AcceptArgs* a, cudaStream_t stream) {
+    if (a->S <= 0) return 0;
+    if (a->depth <= 0) return mllm_fail(1, "accept_drafts: paths of %lld rows", a->depth);
+    if (a->logits && a->T > 0) {
+        if (a->V <= 0 || a->slices <= 0 || a->T * a->slices > 0x7fffffffLL)
+            return mllm_fail(1, "accept_drafts: vocabulary %lld, %lld rows in %lld slices", a->V, a->T, a->slices);
+        MLLM_CUDA(mllm_launch(accept_scan_kernel, dim3((unsigned)(a->T * a->slices)), dim3(SCAN_THREADS), 0, stream, true, a->logits, a->ld,
+                              (int)a->V, (int)a->slices, a->part_val, a->part_idx));
     }
-    MLLM_CUDA(mllm_launch(accept_walk_kernel, dim3(S), dim3(MAX_NODES), 0, stream, true, (const float*)part_val, (const int*)part_idx,
-                          logits ? slices : 0, chosen, tokens, parents, cu_nodes, lengths, path, depth, accepted, next_token,
-                          new_lengths));
+    MLLM_CUDA(mllm_launch(accept_walk_kernel, dim3((unsigned)a->S), dim3(MAX_NODES), 0, stream, true, (const float*)a->part_val,
+                          (const int*)a->part_idx, a->logits ? (int)a->slices : 0, a->chosen, a->tokens, a->parents, a->cu_nodes, a->lengths,
+                          a->path, (int)a->depth, a->accepted, a->next_token, a->new_lengths));
     return 0;
 }
 
 // planes: n_planes x [pages, heads, page_size, row_bytes], plane_bytes apart.
-MLLM_EXPORT int mllm_keep_accepted(void* planes, long long plane_bytes, int n_planes, int pages, int heads, int page_size,
-                                   int row_bytes, const int* block_table, int bt_stride, int width, const int* lengths,
-                                   const int* path, int depth, const int* accepted, int S, cudaStream_t stream) {
-    if (S <= 0 || n_planes <= 0) return 0;
-    if (depth <= 0 || page_size <= 0 || heads <= 0 || row_bytes <= 0 || S > 65535)
-        return mllm_fail(1, "keep_accepted: paths of %d rows, %d heads, pages of %d, rows of %d bytes, %d requests", depth, heads,
-                         page_size, row_bytes, S);
-#define GO(U)                                                                                                                     \
-    do {                                                                                                                          \
-        const long long cols = (long long)n_planes * heads * (row_bytes / (int)sizeof(U));                                        \
-        const int grid = (int)((cols + 127) / 128 < 2048 ? (cols + 127) / 128 : 2048);                                            \
-        MLLM_CUDA(mllm_launch(keep_accepted_kernel<U>, dim3(grid, S), dim3(128), 0, stream, true, (U*)planes,                     \
-                              plane_bytes / (long long)sizeof(U), n_planes, pages, heads, page_size, row_bytes / (int)sizeof(U),  \
-                              block_table, bt_stride, width, lengths, path, depth, accepted));                                    \
-        return 0;                                                                                                                 \
-    } while (0)
-    if (row_bytes % 16 == 0 && (uintptr_t)planes % 16 == 0 && plane_bytes % 16 == 0) GO(uint4);
-    if (row_bytes % 4 == 0 && (uintptr_t)planes % 4 == 0 && plane_bytes % 4 == 0) GO(uint32_t);
-    if (row_bytes % 2 == 0 && (uintptr_t)planes % 2 == 0 && plane_bytes % 2 == 0) GO(uint16_t);
-#undef GO
-    return mllm_fail(1, "keep_accepted: rows of %d bytes", row_bytes);
+struct KeepArgs {
+    void* planes;
+    const int *block_table, *lengths, *path, *accepted;
+    long long plane_bytes, n_planes, pages, heads, page_size, row_bytes, bt_stride, width, depth, S;
+};
+template <typename U>
+static int launch_keep(const KeepArgs* a, cudaStream_t stream) {
+    const long long cols = a->n_planes * a->heads * (a->row_bytes / (int)sizeof(U));
+    const int grid = (int)((cols + 127) / 128 < 2048 ? (cols + 127) / 128 : 2048);
+    MLLM_CUDA(mllm_launch(keep_accepted_kernel<U>, dim3(grid, (unsigned)a->S), dim3(128), 0, stream, true, (U*)a->planes,
+                          a->plane_bytes / (long long)sizeof(U), (int)a->n_planes, (int)a->pages, (int)a->heads, (int)a->page_size,
+                          (int)(a->row_bytes / (int)sizeof(U)), a->block_table, (int)a->bt_stride, (int)a->width, a->lengths, a->path,
+                          (int)a->depth, a->accepted));
+    return 0;
+}
+MLLM_EXPORT int mllm_keep_accepted(const KeepArgs* a, cudaStream_t stream) {
+    if (a->S <= 0 || a->n_planes <= 0) return 0;
+    if (a->depth <= 0 || a->page_size <= 0 || a->heads <= 0 || a->row_bytes <= 0 || a->S > 65535)
+        return mllm_fail(1, "keep_accepted: paths of %lld rows, %lld heads, pages of %lld, rows of %lld bytes, %lld requests", a->depth, a->heads,
+                         a->page_size, a->row_bytes, a->S);
+    const unsigned long long bits = (unsigned long long)a->row_bytes | (uintptr_t)a->planes | (unsigned long long)a->plane_bytes;
+    if (bits % 16 == 0) return launch_keep<uint4>(a, stream);
+    if (bits % 4 == 0) return launch_keep<uint32_t>(a, stream);
+    if (bits % 2 == 0) return launch_keep<uint16_t>(a, stream);
+    return mllm_fail(1, "keep_accepted: rows of %lld bytes", a->row_bytes);
 }

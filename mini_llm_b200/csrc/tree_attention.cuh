@@ -15,18 +15,24 @@ struct Args {
     const int* lengths; const int* cu_nodes; const int* ancestors; int words;
     void* out; long long ldo;
     float* part_o; float* part_ml;          // [2 * blocks, tile rows, dh] and [2 * blocks, tile rows, 2]
+    struct Cut* cuts;                       // [blocks]
     int S, H, Hkv, G, dh, page_size, page_shift;
     int q_vec, out_vec;                     // queries can be read 16 bytes at a time; elements that a store may write at once
     int tile_rows, tile_shift, max_rows;    // query rows of a tile (a power of two), and those of the largest tree's first
-    int unit_shift, blocks, max_tiles;      // keys per unit of work and blocks that share the line of units; 0: a block per pair
+    int unit_shift, least, blocks;          // keys per unit of work, the least of them for a block, blocks (0: one per pair)
+    int max_tiles;
     float scale_log2;
 };
+
+// A pair of query rows and head that the boundary before block c cuts, if no earlier boundary does (else parts is 0): where its rows
+// go, and whose sums they are.  Block c writes it, the join kernel reads it.
+struct Cut { int parts, first, hk, row0, rows, slot, shift, unused; };      // slot: of part 0 less shift; part p > 0 has slot + 2 p
 
 // ------------------------------------------------------------------------------------------------ how the work is cut
 // A pair is a tile of query rows of one (request, key/value head).  Either every pair has a block of its own (blocks == 0: the grid
 // is (head and tile, request)), or the pairs' keys are shared out evenly: each pair's keys in units of 2^unit_shift, all units of all pairs
 // in one line, in order of request, head, tile and position, and every block takes as many neighbours of that line as any other
-// (or one less), whatever the lengths.  A block's share of one pair is a segment.  Pairs that lie in one block are finished there;
+// (or one less), whatever the lengths, but no fewer than its groups or streams can walk at once.  A block's share of one pair is a segment.  Pairs that lie in one block are finished there;
 // the others leave their segments' sums in scratch, two slots a block (only its first and last segment can be parts of a pair), and
 // the join kernel adds them in order of position.  A
 // block finds its place by a scan over the requests, 32 at a time.
@@ -51,9 +57,9 @@ __device__ __forceinline__ Request request_of(const Args& a, int s) {
 __device__ __forceinline__ unsigned int weight_of(const Args& a, const Request& r) { return (unsigned int)r.units * r.tiles * a.Hkv; }
 
 struct Line {                               // the line of units, shared out among blocks: the first `extra` of them take per + 1
-    unsigned int units, per, extra;
+    unsigned int units, blocks, per, extra;
     Request mine;                           // the lane's request among the first 32
-    __device__ __forceinline__ unsigned int begin(unsigned int c) const { return c * per + min(c, extra); }
+    __device__ __forceinline__ unsigned int begin(unsigned int c) const { return c < blocks ? c * per + min(c, extra) : units; }
     __device__ __forceinline__ unsigned int block_of(unsigned int u) const {
         const unsigned int head = extra * (per + 1);
         return u < head ? u / (per + 1) : extra + (u - head) / per;
@@ -65,8 +71,10 @@ __device__ __forceinline__ Line line_of(const Args& a) {       // all lanes of a
     unsigned int sum = weight_of(a, l.mine);
     for (int s = 32 + (threadIdx.x & 31); s < a.S; s += 32) sum += weight_of(a, request_of(a, s));
     l.units = __reduce_add_sync(0xffffffffu, sum);
-    l.per = l.units / a.blocks;
-    l.extra = l.units % a.blocks;
+    const unsigned int blocks = max(1u, min((unsigned int)a.blocks, l.units / a.least));
+    l.per = l.units / blocks;
+    l.extra = l.units % blocks;
+    l.blocks = blocks;
     return l;
 }
 // The request that unit u belongs to, and the first unit of that request; all lanes together.
@@ -123,7 +131,9 @@ __device__ __forceinline__ void fill(const Args& a, Segments* l) {              
     } else {
         const Line line = line_of(a);
         const unsigned int begin = line.begin(blockIdx.x), end = line.begin(blockIdx.x + 1);
-        if (at == 0xffffffffu) at = begin;
+        const bool opening = at == 0xffffffffu;
+        if (opening) at = begin;
+        if (opening && begin >= end && lane == 0) a.cuts[blockIdx.x].parts = 0;
         unsigned int base = 0;
         Request r{};
         bool have = false;
@@ -132,6 +142,15 @@ __device__ __forceinline__ void fill(const Args& a, Segments* l) {              
             have = true;
             const unsigned int pair = (at - base) / r.units, unit = at - base - pair * r.units, take = min(r.units - unit, end - at);
             const unsigned int hk = pair / r.tiles;
+            if (opening && at == begin && lane == 0) {
+                const unsigned int from = at - unit, c0 = blockIdx.x - 1;
+                Cut cut{0, r.first, (int)hk, (int)(pair - hk * r.tiles) * a.tile_rows, r.n * a.G, 2 * (int)c0, 0, 0};
+                if (unit && line.begin(c0) <= from) {
+                    cut.parts = (int)(line.block_of(from + r.units - 1) - c0) + 1;
+                    cut.shift = line.begin(c0) < from ? 1 : 0;        // block c0's segment is its last one, unless it begins with it
+                }
+                a.cuts[blockIdx.x] = cut;
+            }
             if (lane == 0)
                 l->list[count] = Segment{r.s, r.first, r.n, r.len, r.keys, (int)hk, (int)(pair - hk * r.tiles) * a.tile_rows, r.n * a.G,
                                          (int)(unit << a.unit_shift), (int)min((long long)(unit + take) << a.unit_shift, (long long)r.keys),
@@ -182,9 +201,26 @@ __device__ __forceinline__ float fast_exp2(float x) {
 
 inline dim3 grid_of(const Args& a) { return a.blocks ? dim3(a.blocks) : dim3(a.Hkv * a.max_tiles, a.S); }
 
+// Rows of a TMA box: the largest power of two that divides a page, at most a tile's.  Boxes of 8 rows and more keep the pattern of the
+// 128-byte swizzle, which repeats every 8.
+inline int box_rows(int page_size, int tile) {
+    while (page_size % tile) tile >>= 1;
+    return tile;
+}
+inline bool boxes_ok(const Args& a, long long pages) {
+    return a.page_size % 8 == 0 && pages * a.Hkv * a.page_size + 64 <= 0x7fffffffLL;
+}
+
 // Adds the segments of the pairs that were cut (tree_attention.cu).
 int join(const Args& a, int dtype, cudaStream_t stream);
+// float32 (tree_attention_f32.cu).  info not null: only describes the variant.
+int f32(const Args* a, int dh, long long pages, int tile_rows, int wide, int* info, cudaStream_t stream);
 // bfloat16 on the fifth-generation tensor cores, tiles of 128 or 256 rows (tree_attention_tcgen05.cu).
 int tcgen05(const Args& a, long long pages, cudaStream_t stream);
+int tcgen05_variant(int dh, int tile_rows, int* info);
+int bind_error_f32(int* word);
+int bind_error_tcgen05(int* word);
+int error_f32(int* code);
+int error_tcgen05(int* code);
 
 }  // namespace tree

@@ -547,22 +547,25 @@ int launch(const Args& a, const CUtensorMap& mk, const CUtensorMap& mv, int box,
 
 }  // namespace
 
-// The pinned host word that this file's kernels write when they give up on a wait.
-MLLM_EXPORT int mllm_tree_attention_bind_error(int* word) { return bind_host_error(word); }
-
-// The first error recorded by the kernel since the last call (0 = none); resets it.
-MLLM_EXPORT int mllm_tree_attention_error(int* code) {
+int tree::bind_error_tcgen05(int* word) { return bind_host_error(word); }
+int tree::error_tcgen05(int* code) {
     int zero = 0;
     MLLM_CUDA(cudaMemcpyFromSymbol(code, g_tree_error, sizeof(int)));
     if (*code) MLLM_CUDA(cudaMemcpyToSymbol(g_tree_error, &zero, sizeof(int)));
     return 0;
 }
 
+int tree::tcgen05_variant(int dh, int tile_rows, int* info) {
+    if (dh > 128 || (tile_rows != BQ && tile_rows != 2 * BQ)) return mllm_fail(1, "tree_attention: the tcgen05 kernel takes no tiles of %d rows of heads of %d", tile_rows, dh);
+    info[0] = 1;
+    info[1] = BKV * (dh <= 64 ? (tile_rows == BQ ? Plan<64, 1>::KS : Plan<64, 2>::KS) : (tile_rows == BQ ? Plan<128, 1>::KS : Plan<128, 2>::KS));
+    return 0;
+}
+
 int tree::tcgen05(const Args& a, long long pages, cudaStream_t stream) {
     const long long rows = pages * a.Hkv * a.page_size;
-    int box = 64;
-    while (a.page_size % box) box >>= 1;
-    if (a.dh > 128 || box < 8 || rows + 64 > 0x7fffffffLL || (a.tile_rows != BQ && a.tile_rows != 2 * BQ))
+    const int box = tree::box_rows(a.page_size, BKV);
+    if (a.dh > 128 || !tree::boxes_ok(a, pages) || (a.tile_rows != BQ && a.tile_rows != 2 * BQ))
         return mllm_fail(1, "tree_attention: the tcgen05 kernel takes heads of up to 128, pages of a multiple of 8 tokens and "
                             "tiles of 128 or 256 rows, not %d, %d, %d", a.dh, a.page_size, a.tile_rows);
     CUtensorMap mk, mv;

@@ -1,0 +1,634 @@
+// The kernel of tree attention on tiles of keys in shared memory; tree_attention.cu says what it does, and instantiates it for
+// bfloat16, tree_attention_f32.cu for float32.
+#pragma once
+#include "tcgen05.cuh"
+#include "tree_attention.cuh"
+#include <type_traits>
+
+namespace {
+
+using namespace tree;
+
+__device__ int g_tiles_error = 0;                           // first error code seen by this file's kernels
+__device__ __forceinline__ void report(int code) {
+    atomicCAS(&g_tiles_error, 0, 20 + code);
+    tc::report_to_host(1020 + code);
+}
+
+__device__ __forceinline__ uint32_t s_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
+    const int n = valid ? 16 : 0;                     // 0 source bytes: the 16 bytes are filled with zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s_u32(dst)), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s_u32(p)) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s_u32(p)) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+// Two fused multiply-adds of neighbouring 32-bit floats in one instruction.
+__device__ __forceinline__ void fma2(unsigned long long& c, unsigned long long a, unsigned long long b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ unsigned long long pair_of(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float2 halves(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+// The warps of one group; one warp needs no barrier of the block.
+template <int WR> __device__ __forceinline__ void group_sync(int group) {
+    if (WR == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(WR * 32) : "memory");
+}
+template <int WR> __device__ __forceinline__ bool group_any(int group, bool x) {
+    if (WR == 1) return __any_sync(0xffffffffu, x);
+    int r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+                 "barrier.cta.red.or.pred q, %2, %3, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"((int)x), "r"(group + 1), "n"(WR * 32) : "memory");
+    return r != 0;
+}
+
+constexpr int P_ROW = 36;                                   // float32: a row of weights, padded so that 4 rows start on other banks
+
+template <typename T, int DP, int RW, int WR, int WK, int BK, int ST>
+struct Shape {
+    static constexpr int VEC = 16 / sizeof(T);
+    static constexpr int ROW = DP + VEC;                    // a query row, padded: neighbours start on other banks
+    static constexpr int CB = DP * (int)sizeof(T) / 128;    // blocks of 128 bytes in a key row
+    static constexpr int TILE = BK * DP;                    // elements of a buffer: [CB][BK][128 bytes], 16-byte pieces swizzled by row
+    static constexpr int ROWS = RW * WR;
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr size_t q_bytes = (size_t)ROWS * ROW * sizeof(T);
+    static constexpr size_t kv_bytes = (size_t)WK * ST * 2 * TILE * sizeof(T);
+    static constexpr size_t p_bytes = F32 ? (size_t)WK * WR * RW * P_ROW * 4 : 0;
+    static constexpr int MN = F32 ? RW / 4 : 2;             // rows whose maximum and sum a thread keeps
+    static constexpr int ON = F32 ? RW / 4 * (DP / 8) : DP / 2;
+    static constexpr int X_ROW = DP + 8;                    // the groups' results meet as rows of 32-bit floats
+    static constexpr size_t xch_bytes = WK > 1 ? (size_t)WK * ROWS * (X_ROW + 2) * 4 : 0;
+    static constexpr size_t bytes = (kv_bytes + p_bytes > xch_bytes ? kv_bytes + p_bytes : xch_bytes) + q_bytes;
+};
+
+template <typename T, int DP, int RW, int WR, int WK, int BK, int ST, int PER_SM, bool TMA>
+__global__ void __launch_bounds__(WR * WK * 32, PER_SM)
+tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, int box, int pool_rows) {
+    using S = Shape<T, DP, RW, WR, WK, BK, ST>;
+    constexpr int VEC = S::VEC, ROW = S::ROW, CH = DP / VEC, NT = WR * 32, MN = S::MN, ON = S::ON, TILE = S::TILE;
+    constexpr bool F32 = S::F32;
+    using mask_t = typename std::conditional<BK == 32, uint32_t, unsigned long long>::type;
+    extern __shared__ __align__(1024) uint8_t smem[];       // buffers first: the swizzle goes by the address
+    __shared__ uint64_t k_full[TMA ? WK : 1][ST], v_full[TMA ? WK : 1][ST];
+    __shared__ int s_failed;
+    volatile int* failed = &s_failed;
+    const int group = threadIdx.x / NT, gtid = threadIdx.x % NT, warp = gtid >> 5, lane = gtid & 31;
+    T* sK = reinterpret_cast<T*>(smem) + (size_t)group * ST * 2 * TILE;
+    T* sV = sK + ST * TILE;
+    float* sP = reinterpret_cast<float*>(smem + S::kv_bytes) + (size_t)(group * WR + warp) * RW * P_ROW;
+    T* sQ = reinterpret_cast<T*>(smem + S::bytes - S::q_bytes);
+    // element `d` of a buffer's row: 16-byte pieces of a block of 128 bytes stand in an order of the row's own
+    auto at = [&](const T* buffer, int row, int d) {
+        const int piece = d / VEC;
+        return buffer + (piece >> 3) * (BK * 128 / (int)sizeof(T)) + row * (128 / (int)sizeof(T)) + ((piece ^ row) & 7) * VEC + d % VEC;
+    };
+    if (TMA && threadIdx.x == 0) {
+        for (int w = 0; w < WK; ++w)
+            for (int st = 0; st < ST; ++st) { tc::mbar_init(&k_full[w][st], 1); tc::mbar_init(&v_full[w][st], 1); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tc::prefetch_map(&map_k);
+        tc::prefetch_map(&map_v);
+    }
+    if (threadIdx.x == 0) s_failed = TMA && (s_u32(smem) & 1023) ? 2 : 0;
+
+    pdl_wait();
+    pdl_launch();
+    const int G = a.G;
+    const T* k_pages = static_cast<const T*>(a.k_pages);
+    const T* v_pages = static_cast<const T*>(a.v_pages);
+    const int dh_ch = a.dh / VEC;                           // 16-byte pieces of a row; the rest of DP is zeros
+
+    __shared__ Segments segments;
+    bool dead = false;                                      // this thread has given up waiting
+    int uses = 0;                                           // of this group's buffers so far: the phase of their barriers
+    if (threadIdx.x == 0) first_segments(&segments);
+    for (int number = 0;; ++number) {
+        if (number % Segments::CAP == 0) {
+            if (number && !segments.more) break;
+            __syncthreads();
+            if (threadIdx.x < 32) fill(a, &segments);
+            __syncthreads();
+        }
+        if (number % Segments::CAP >= segments.count || *failed == 2) break;
+        const Segment& sg = segments.list[number % Segments::CAP];
+        const int first = sg.first, len = sg.len, keys = sg.keys, rows = sg.rows, r0 = sg.row0, hk = sg.hk, k1 = sg.k1;
+        const int* bt = a.block_table + (size_t)sg.s * a.bt_stride;
+        const int t_last = (k1 - 1) / BK;                   // units are multiples of a tile
+        const bool active = r0 + warp * RW < rows;          // a warp without rows only helps with the copies
+
+        // What a lane looks up of a tile, ahead of its copies: TMA, the page on which its box starts; else those of the tile's keys
+        // lane, lane + 32.  The arithmetic waits until the copies are made (a use behind the load would hold the warp up).
+        constexpr int LOOKS = TMA ? 1 : BK / 32;
+        int page[LOOKS], place[LOOKS];                        // place: the row within the page, -1 past the segment
+        auto look_up = [&](int t) {
+#pragma unroll
+            for (int x = 0; x < LOOKS; ++x) {
+                const int kp = t * BK + (TMA ? lane * box : x * 32 + lane);
+                place[x] = -1;
+                if (kp < k1 && (!TMA || lane * box < BK)) {
+                    const int p = a.page_shift >= 0 ? kp >> a.page_shift : kp / a.page_size;
+                    place[x] = kp - p * a.page_size;
+                    page[x] = bt[p];
+                }
+            }
+        };
+        auto row_of_look = [&](int x) -> unsigned int {
+            return place[x] < 0 ? (TMA ? (unsigned int)pool_rows : NO_ROW) : ((unsigned int)page[x] * a.Hkv + hk) * a.page_size + place[x];
+        };
+        auto load = [&](T* dst, const T* pages, const CUtensorMap* map, uint64_t* bar) {       // the rows that look_up() brought
+            if constexpr (TMA) {
+                if (warp != 0) return;
+                const int row = (int)row_of_look(0);          // beyond the pool, i.e. zeros, past the segment
+                if (lane == 0) tc::mbar_expect_tx(bar, TILE * sizeof(T));
+                __syncwarp();
+                if (lane * box < BK) {
+#pragma unroll 1
+                    for (int c = 0; c < S::CB; ++c)
+                        tc::tma_load_2d(reinterpret_cast<uint8_t*>(dst) + c * (BK * 128) + lane * box * 128, map, c * (128 / (int)sizeof(T)),
+                                        row, bar);
+                }
+            } else {
+                unsigned int row_id[LOOKS];
+#pragma unroll
+                for (int x = 0; x < LOOKS; ++x) row_id[x] = row_of_look(x);
+#pragma unroll
+                for (int it = 0; it < BK * CH / NT; ++it) {
+                    const int i = gtid + it * NT, r = i / CH, c = i % CH;
+                    unsigned int id = __shfl_sync(0xffffffffu, row_id[0], r & 31);
+                    if (BK > 32) {
+                        const unsigned int other = __shfl_sync(0xffffffffu, row_id[LOOKS - 1], r & 31);
+                        id = r >= 32 ? other : id;
+                    }
+                    const bool ok = id != NO_ROW && c < dh_ch;
+                    cp_async16(const_cast<T*>(at(dst, r, c * VEC)), pages + (ok ? (size_t)id * a.dh + c * VEC : 0), ok);
+                }
+            }
+        };
+        // a buffer's copies are there (for this thread's own, where it made them: a barrier of the group follows)
+        auto wait = [&](uint64_t* bar, int use) {
+            if constexpr (TMA) {
+                if (!dead && !tc::mbar_wait(bar, (use / ST) & 1)) { dead = true; *failed = 1; }
+            } else {
+                cp_wait<2 * ST - 1>();
+            }
+        };
+        int t = sg.k0 / BK + group;
+        look_up(t);
+        // the queries of this tile of rows
+        const T* q = static_cast<const T*>(a.q);
+#pragma unroll 1
+        for (int i = threadIdx.x; i < S::ROWS * CH; i += WR * WK * 32) {
+            const int r = i / CH, c = i % CH;
+            const bool ok = r0 + r < rows && c < dh_ch;
+            const int node = ok ? (r0 + r) / G : 0, h = hk * G + (ok ? (r0 + r) % G : 0);
+            const T* src = q + (size_t)(first + node) * a.ldq + (size_t)h * a.dh + c * VEC;
+            if (a.q_vec) {
+                cp_async16(sQ + r * ROW + c * VEC, ok ? src : q, ok);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) sQ[r * ROW + c * VEC + e] = ok ? src[e] : from_f32<T>(0.f);
+            }
+        }
+        cp_commit();
+
+#pragma unroll
+        for (int st = 0; st < ST; ++st) {
+            const int buf = TMA ? (uses + st) % ST : st;
+            if (st) look_up(t + st * WK);
+            if (t + st * WK <= t_last) load(sK + buf * TILE, k_pages, &map_k, &k_full[TMA ? group : 0][buf]);
+            if (!TMA) cp_commit();
+            if (t + st * WK <= t_last) load(sV + buf * TILE, v_pages, &map_v, &v_full[TMA ? group : 0][buf]);
+            if (!TMA) cp_commit();
+        }
+        look_up(t + ST * WK);
+        if (TMA) cp_wait<0>();
+        else cp_wait<2 * ST>();                               // the queries are in
+        __syncthreads();
+
+        // ---- running state
+        float o[F32 ? 1 : ON];                                // bfloat16: the accumulators' fragments
+        unsigned long long o2[F32 ? ON / 2 : 1];              // float32: [MN][DP / 32][2] pairs of columns
+#pragma unroll
+        for (int i = 0; i < (F32 ? 1 : ON); ++i) o[i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < (F32 ? ON / 2 : 1); ++i) o2[i] = 0ull;
+        float m_run[MN], l_run[MN];
+#pragma unroll
+        for (int i = 0; i < MN; ++i) { m_run[i] = -INFINITY; l_run[i] = 0.f; }
+        const int g = lane >> 2, tq = lane & 3;               // bfloat16: fragment row and column
+        const int rg = lane >> 3, kg = lane & 7;              // float32: row and key (or column) of a lane
+        uint32_t qa[F32 ? 1 : DP / 16][4];
+        if constexpr (!F32) {
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) ldsm_x4(qa[ks], sQ + (warp * 16 + (lane & 15)) * ROW + ks * 16 + (lane >> 4) * 8);
+        }
+        auto row_of = [&](int i) { return r0 + warp * RW + (F32 ? rg + 4 * i : g + 8 * i); };      // the query row of a thread's i-th state
+        auto words_of = [&](int r) { return a.ancestors + (size_t)(first + (r < rows ? r / G : 0)) * a.words; };
+
+        for (int use = TMA ? uses : 0; t <= t_last; t += WK, ++use) {
+            const int stage = use % ST;
+            T* tK = sK + stage * TILE;
+            T* tV = sV + stage * TILE;
+            const int key0 = t * BK;
+            const bool tail = key0 + BK > min(len, keys);     // the tile reaches into the tree or past the keys
+            mask_t seen[MN];
+            if (tail) {
+#pragma unroll
+                for (int i = 0; i < MN; ++i)
+                    seen[i] = (mask_t)tile_mask(words_of(row_of(i)), a.words, len, keys, key0, row_of(i) < rows);
+            }
+            wait(&k_full[TMA ? group : 0][stage], use);       // the tile's keys
+            if (!TMA || WR > 1) group_sync<WR>(group);
+            float sc[F32 ? 4 * MN : BK / 2];                  // scores, then weights
+            if (active) {
+                if constexpr (!F32) {
+                    // ---- S = Q K^T: 16 rows x BK keys
+#pragma unroll
+                    for (int i = 0; i < BK / 2; ++i) sc[i] = 0.f;
+#pragma unroll
+                    for (int ks = 0; ks < DP / 16; ++ks) {
+#pragma unroll
+                        for (int np = 0; np < BK / 16; ++np) {
+                            uint32_t b[4];
+                            ldsm_x4(b, at(tK, np * 16 + (lane & 7) + ((lane >> 4) << 3), ks * 16 + ((lane >> 3) & 1) * 8));
+                            mma16816(*reinterpret_cast<float (*)[4]>(&sc[8 * np]), qa[ks], b[0], b[1]);
+                            mma16816(*reinterpret_cast<float (*)[4]>(&sc[8 * np + 4]), qa[ks], b[2], b[3]);
+                        }
+                    }
+                } else {
+                    // ---- S: rows rg + 4 i, keys kg + 8 j; even and odd columns in the halves of a pair
+                    unsigned long long s2[MN][4];
+#pragma unroll
+                    for (int i = 0; i < MN; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s2[i][j] = 0ull;
+                    const float* qr = reinterpret_cast<const float*>(sQ) + (warp * RW + rg) * ROW;
+#pragma unroll 4
+                    for (int d = 0; d < DP; d += 4) {
+                        ulonglong2 qv[MN];
+#pragma unroll
+                        for (int i = 0; i < MN; ++i) qv[i] = *reinterpret_cast<const ulonglong2*>(qr + 4 * i * ROW + d);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const ulonglong2 kv = *reinterpret_cast<const ulonglong2*>(at(tK, kg + 8 * j, d));
+#pragma unroll
+                            for (int i = 0; i < MN; ++i) { fma2(s2[i][j], qv[i].x, kv.x); fma2(s2[i][j], qv[i].y, kv.y); }
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < MN; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) { const float2 h = halves(s2[i][j]); sc[4 * i + j] = h.x + h.y; }
+                }
+            }
+            group_sync<WR>(group);                            // the keys' buffer is free
+            if (t + ST * WK <= t_last) load(tK, k_pages, &map_k, &k_full[TMA ? group : 0][stage]);
+            if (!TMA) cp_commit();
+
+            if (active) {
+                // ---- weights, and what they do to the state
+                float alpha[MN];
+                bool moved = false;
+#pragma unroll
+                for (int i = 0; i < MN; ++i) {
+                    float mx = -INFINITY;
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (tail && !(seen[i] >> (kg + 8 * j) & 1)) sc[4 * i + j] = -INFINITY;
+                            mx = fmaxf(mx, sc[4 * i + j]);
+                        }
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    } else {
+#pragma unroll
+                        for (int nt = 0; nt < BK / 8; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                if (tail && !(seen[i] >> (nt * 8 + 2 * tq + e) & 1)) sc[4 * nt + 2 * i + e] = -INFINITY;
+                                mx = fmaxf(mx, sc[4 * nt + 2 * i + e]);
+                            }
+                    }
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    const float m_new = fmaxf(m_run[i], mx), use = m_new == -INFINITY ? 0.f : m_new;
+                    if constexpr (F32) {
+                        alpha[i] = exp2f((m_run[i] - use) * a.scale_log2);
+                        float sum = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float p = exp2f((sc[4 * i + j] - use) * a.scale_log2);
+                            sP[(rg + 4 * i) * P_ROW + kg + 8 * j] = p;
+                            sum += p;
+                        }
+                        l_run[i] = l_run[i] * alpha[i] + sum;          // this lane's keys; the lanes meet at the end
+                    } else {
+                        alpha[i] = fast_exp2((m_run[i] - use) * a.scale_log2);
+                        const unsigned long long neg = pair_of(-use, -use), scale2 = pair_of(a.scale_log2, a.scale_log2);
+                        unsigned long long sum = 0ull;
+#pragma unroll
+                        for (int nt = 0; nt < BK / 8; ++nt) {
+                            float &p0 = sc[4 * nt + 2 * i], &p1 = sc[4 * nt + 2 * i + 1];
+                            const float2 x = halves(mul2(add2(pair_of(p0, p1), neg), scale2));
+                            p0 = fast_exp2(x.x);
+                            p1 = fast_exp2(x.y);
+                            sum = add2(sum, pair_of(p0, p1));
+                        }
+                        const float2 both = halves(sum);
+                        l_run[i] = l_run[i] * alpha[i] + (both.x + both.y);
+                    }
+                    moved |= alpha[i] != 1.f;
+                    m_run[i] = m_new;
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int i = 0; i < MN; ++i)
+#pragma unroll
+                            for (int c = 0; c < DP / 16; ++c) {
+                                const float2 h = halves(o2[i * (DP / 16) + c]);
+                                o2[i * (DP / 16) + c] = pair_of(h.x * alpha[i], h.y * alpha[i]);
+                            }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < ON; ++i) o[i] *= alpha[i >> 1 & 1];
+                    }
+                }
+            }
+
+            wait(&v_full[TMA ? group : 0][stage], use);       // the tile's values
+            bool odd = false;
+            if (tail) {
+                // values past the last key (boxes bring whole ones), and infinite and NaN ones of the tree: out, before the group
+                // reads the tile
+                if (!TMA) group_sync<WR>(group);
+#pragma unroll 1
+                for (int i = gtid; i < BK * CH; i += NT) {
+                    const int r = i / CH;
+                    if (key0 + r < min(len, keys)) continue;
+                    uint4* w = reinterpret_cast<uint4*>(const_cast<T*>(at(tV, r, i % CH * VEC)));
+                    if (key0 + r >= keys) *w = make_uint4(0u, 0u, 0u, 0u);
+                    else if (odd_element<T>(w->x) || odd_element<T>(w->y) || odd_element<T>(w->z) || odd_element<T>(w->w)) {
+                        *w = make_uint4(without_odd<T>(w->x), without_odd<T>(w->y), without_odd<T>(w->z), without_odd<T>(w->w));
+                        odd = true;
+                    }
+                }
+                if (TMA) tc::fence_async_smem();              // the next tile comes the other way
+                odd = group_any<WR>(group, odd);
+            }
+            if (!TMA || WR > 1 || tail) group_sync<WR>(group);
+            if (active) {
+                // ---- O += P V
+                if constexpr (!F32) {
+#pragma unroll
+                    for (int kk = 0; kk < BK / 16; ++kk) {
+                        uint32_t pa[4], pb[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float p0 = sc[8 * kk + 2 * e], p1 = sc[8 * kk + 2 * e + 1];
+                            pa[e] = pack_bf16(p0, p1);
+                            pb[e] = pack_bf16(p0 - __uint_as_float(pa[e] << 16), p1 - __uint_as_float(pa[e] & 0xffff0000u));
+                        }
+#pragma unroll
+                        for (int dp = 0; dp < DP / 16; ++dp) {
+                            uint32_t b[4];
+                            ldsm_x4_trans(b, at(tV, kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, dp * 16 + (lane >> 4) * 8));
+                            float (&c0)[4] = *reinterpret_cast<float (*)[4]>(&o[8 * dp]);
+                            float (&c1)[4] = *reinterpret_cast<float (*)[4]>(&o[8 * dp + 4]);
+                            mma16816(c0, pa, b[0], b[1]);
+                            mma16816(c1, pa, b[2], b[3]);
+                            mma16816(c0, pb, b[0], b[1]);
+                            mma16816(c1, pb, b[2], b[3]);
+                        }
+                    }
+                } else {
+                    __syncwarp();
+                    const float* pr = sP + rg * P_ROW;
+#pragma unroll 2
+                    for (int k = 0; k < BK; k += 4) {
+                        float4 p[MN];
+#pragma unroll
+                        for (int i = 0; i < MN; ++i) p[i] = *reinterpret_cast<const float4*>(pr + 4 * i * P_ROW + k);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            unsigned long long pp[MN];
+#pragma unroll
+                            for (int i = 0; i < MN; ++i) {
+                                const float x = e == 0 ? p[i].x : e == 1 ? p[i].y : e == 2 ? p[i].z : p[i].w;
+                                pp[i] = pair_of(x, x);
+                            }
+#pragma unroll
+                            for (int c = 0; c < DP / 32; ++c) {
+                                const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(at(tV, k + e, c * 32 + kg * 4));
+#pragma unroll
+                                for (int i = 0; i < MN; ++i) {
+                                    fma2(o2[i * (DP / 16) + 2 * c], pp[i], v.x);
+                                    fma2(o2[i * (DP / 16) + 2 * c + 1], pp[i], v.y);
+                                }
+                            }
+                        }
+                    }
+                }
+                if (tail && odd) {
+                    // infinite and NaN elements, from memory, to the rows that see them
+                    for (int b = max(0, len - key0); b < min(BK, k1 - key0); ++b) {
+                        const int kp = key0 + b, p = kp / a.page_size;
+                        const T* vrow = v_pages + (((size_t)bt[p] * a.Hkv + hk) * a.page_size + kp % a.page_size) * a.dh;
+#pragma unroll
+                        for (int i = 0; i < MN; ++i) {
+                            if (!(seen[i] >> b & 1)) continue;
+#pragma unroll
+                            for (int e = 0; e < (F32 ? DP / 16 : DP / 8); ++e) {
+                                const int d = F32 ? (e >> 1) * 32 + kg * 4 + 2 * (e & 1) : e * 8 + 2 * tq;
+                                if (d >= a.dh) continue;
+                                float x = to_f32(vrow[d]), y = to_f32(vrow[d + 1]);
+                                x = fabsf(x) < INFINITY ? 0.f : x;
+                                y = fabsf(y) < INFINITY ? 0.f : y;
+                                if constexpr (F32) {
+                                    const float2 h = halves(o2[i * (DP / 16) + e]);
+                                    o2[i * (DP / 16) + e] = pair_of(h.x + x, h.y + y);
+                                } else {
+                                    o[e * 4 + 2 * i] += x;
+                                    o[e * 4 + 2 * i + 1] += y;
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            group_sync<WR>(group);                            // the values' buffer is free
+            if (t + ST * WK <= t_last) load(tV, v_pages, &map_v, &v_full[TMA ? group : 0][stage]);
+            if (!TMA) cp_commit();
+            look_up(t + (ST + 1) * WK);
+            if (TMA) uses = use + 1;
+        }
+        if (!TMA) cp_wait<0>();
+        // the lanes' shares of the sums
+#pragma unroll
+        for (int i = 0; i < MN; ++i) {
+            if (F32) l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 4);
+            l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
+            l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
+        }
+        float res[ON];                                        // [MN][columns], a pair of neighbours after the other
+#pragma unroll
+        for (int i = 0; i < MN; ++i)
+#pragma unroll
+            for (int e = 0; e < ON / MN / 2; ++e) {
+                if constexpr (F32) {
+                    const float2 h = halves(o2[i * (DP / 16) + e]);
+                    res[i * (ON / MN) + 2 * e] = h.x;
+                    res[i * (ON / MN) + 2 * e + 1] = h.y;
+                } else {
+                    res[i * (ON / MN) + 2 * e] = o[e * 4 + 2 * i];
+                    res[i * (ON / MN) + 2 * e + 1] = o[e * 4 + 2 * i + 1];
+                }
+            }
+        // ---- out: a thread's own elements where the block is one group; else the groups' rows meet in shared memory, in order, and
+        // every thread finishes neighbours of a row
+        auto put = [&](int r, int d, float x, float y, float m, float l, bool first_of_row) {
+            if (sg.slot >= 0) {
+                const size_t pr = (size_t)sg.slot * a.tile_rows + (r - r0);
+                if (first_of_row) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = make_float2(m, l);
+                *reinterpret_cast<float2*>(a.part_o + pr * a.dh + d) = make_float2(x, y);
+                return;
+            }
+            const float inv = inverse_sum(l);
+            T* orow = static_cast<T*>(a.out) + (size_t)(first + r / G) * a.ldo + (size_t)(hk * G + r % G) * a.dh;
+            if (F32 && a.out_vec >= 2) *reinterpret_cast<float2*>(orow + d) = make_float2(x * inv, y * inv);
+            else if (!F32 && a.out_vec >= 2) *reinterpret_cast<uint32_t*>(orow + d) = pack_bf16(x * inv, y * inv);
+            else { orow[d] = from_f32<T>(x * inv); orow[d + 1] = from_f32<T>(y * inv); }
+        };
+        if constexpr (WK > 1) {
+            constexpr int X = S::X_ROW;
+            float* xch = reinterpret_cast<float*>(smem);                   // [WK][ROWS][X], then maxima and sums [WK][ROWS][2]
+            float* xml = xch + WK * S::ROWS * X;
+            __syncthreads();
+            if (active) {
+#pragma unroll
+                for (int i = 0; i < MN; ++i) {
+                    const int r = group * S::ROWS + row_of(i) - r0;
+                    if ((F32 ? kg : tq) == 0) *reinterpret_cast<float2*>(xml + 2 * r) = make_float2(m_run[i], l_run[i]);
+#pragma unroll
+                    for (int e = 0; e < ON / MN / 2; ++e) {
+                        const int d = F32 ? (e >> 1) * 32 + kg * 4 + 2 * (e & 1) : e * 8 + 2 * tq;
+                        *reinterpret_cast<float2*>(xch + r * X + d) = make_float2(res[i * (ON / MN) + 2 * e], res[i * (ON / MN) + 2 * e + 1]);
+                    }
+                }
+            }
+            __syncthreads();
+            const int pairs = a.dh / 2, here = min(S::ROWS, rows - r0);
+            for (int i = threadIdx.x; i < here * pairs; i += WR * WK * 32) {
+                const int r = i / pairs, d = 2 * (i % pairs);
+                float2 ml[WK];
+                float m = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    ml[w] = *reinterpret_cast<const float2*>(xml + 2 * (w * S::ROWS + r));
+                    m = fmaxf(m, ml[w].x);
+                }
+                const float use = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    const float f = exp2f((ml[w].x - use) * a.scale_log2);
+                    const float2 v = *reinterpret_cast<const float2*>(xch + (w * S::ROWS + r) * X + d);
+                    l = fmaf(ml[w].y, f, l);
+                    x = fmaf(v.x, f, x);
+                    y = fmaf(v.y, f, y);
+                }
+                put(r0 + r, d, x, y, m, l, d == 0);
+            }
+            if (TMA) tc::fence_async_smem();                  // the next segment's tiles come the other way
+        } else if (active) {
+#pragma unroll
+            for (int i = 0; i < MN; ++i) {
+                const int r = row_of(i);
+                if (r >= rows) continue;
+#pragma unroll
+                for (int e = 0; e < ON / MN / 2; ++e) {
+                    const int d = F32 ? (e >> 1) * 32 + kg * 4 + 2 * (e & 1) : e * 8 + 2 * tq;
+                    if (d < a.dh) put(r, d, res[i * (ON / MN) + 2 * e], res[i * (ON / MN) + 2 * e + 1], m_run[i], l_run[i], d == 0);
+                }
+            }
+        }
+        __syncthreads();                                      // shared memory is free for the next segment
+    }
+    if (TMA) {
+        __syncthreads();
+        if (*failed) {
+            if (threadIdx.x == 0) report(*failed);
+            for (int i = 0; i < 2000; ++i) __nanosleep(100);      // copies already asked for may still be on their way
+        }
+    }
+}
+
+
+template <typename T, int DP, int RW, int WR, int WK, int BK, int ST, int PER_SM, bool TMA>
+int launch(const Args& a, long long pages, cudaStream_t stream) {
+    using Sh = Shape<T, DP, RW, WR, WK, BK, ST>;
+    constexpr size_t fixed = 1024;                          // the segments and barriers, up to the alignment of the buffers
+    static_assert(Sh::bytes + fixed <= 232448 && (Sh::bytes + fixed + 1024) * PER_SM <= 233472, "shared memory of an SM");
+    auto kern = tree_attention_kernel<T, DP, RW, WR, WK, BK, ST, PER_SM, TMA>;
+    static bool set = false;
+    if (!set && Sh::bytes + fixed > 48 * 1024) {
+        MLLM_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::bytes));
+        set = true;
+    }
+    CUtensorMap mk{}, mv{};
+    const int rows = (int)(pages * a.Hkv * a.page_size), box = TMA ? box_rows(a.page_size, BK) : 0;
+    if (TMA) {
+        constexpr int kind = sizeof(T) == 4 ? tc::MAP_F32_SW128 : tc::MAP_BF16_SW128;
+        int rc = tc::get_map(a.k_pages, a.dh, rows, a.dh, 128 / (int)sizeof(T), box, kind, &mk);
+        if (rc) return rc;
+        rc = tc::get_map(a.v_pages, a.dh, rows, a.dh, 128 / (int)sizeof(T), box, kind, &mv);
+        if (rc) return rc;
+    }
+    MLLM_CUDA(mllm_launch(kern, grid_of(a), dim3(WR * WK * 32), Sh::bytes, stream, true, a, mk, mv, box, rows));
+    return a.blocks ? join(a, sizeof(T) == 4 ? MLLM_F32 : MLLM_BF16, stream) : 0;
+}
+
+// One variant, with copies by TMA where the pages allow it.  info not null: only says how many of its blocks an SM holds, and how many
+// keys a block walks at once.
+#define TREE_GO(T, RW, WR, WK, BK, ST, PER)                                                                         \
+    do {                                                                                                            \
+        if (info) { info[0] = PER; info[1] = WK * BK; return 0; }                                                   \
+        return boxes_ok(*a, pages) ? launch<T, DP, RW, WR, WK, BK, ST, PER, true>(*a, pages, stream)                \
+                                   : launch<T, DP, RW, WR, WK, BK, ST, PER, false>(*a, pages, stream);              \
+    } while (0)
+
+}  // namespace

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 import threading
 from typing import Optional
 
@@ -30,7 +31,7 @@ _GATE_ACT = {"gelu_tanh": 1, "gelu_erf": 2, "relu": 3, "silu": 4, "swiglu_clamp"
 _UNGATED_ACT = {"relu_sq": 6}     # activations of one argument that the experts' first product takes (experts without a gate)
 _lib = None
 
-c_int, c_ll, c_float, c_void_p = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
+c_int, c_ll, c_float, c_void_p, c_char_p = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p, ctypes.c_char_p
 
 
 class KernelError(RuntimeError):
@@ -118,19 +119,13 @@ def _signatures(lib):
         "mllm_attention_tiled_wide": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                       c_void_p, c_ll, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
         "mllm_draft_max_nodes": [],
-        "mllm_draft_tables": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
-                              c_void_p, c_void_p, c_void_p, c_int, c_void_p],
+        "mllm_draft_tables": [c_char_p, c_void_p],
         "mllm_tree_attention_bind_error": [c_void_p],
         "mllm_tree_attention_error": [c_void_p],
-        "mllm_tree_attention_per_sm": [c_int, c_int, c_int],
-        "mllm_tree_attention": [c_void_p, c_ll, c_void_p, c_void_p, c_ll, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int,
-                                c_void_p, c_ll, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int,
-                                c_int, c_int, c_int, c_void_p],
-        "mllm_accept_slices": [c_int, c_int],
-        "mllm_accept_drafts": [c_void_p, c_ll, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                               c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
-        "mllm_keep_accepted": [c_void_p, c_ll, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int,
-                               c_void_p, c_int, c_void_p],
+        "mllm_tree_attention_variant": [c_int, c_int, c_int, c_int, c_void_p],
+        "mllm_tree_attention": [c_char_p, c_void_p],
+        "mllm_accept_drafts": [c_char_p, c_void_p],
+        "mllm_keep_accepted": [c_char_p, c_void_p],
         "mllm_rmsnorm": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_int, c_int, c_int, c_float,
                          c_float, c_float, c_int, c_void_p],
         "mllm_gated_recurrence_wide": [c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_void_p, c_void_p,
@@ -398,7 +393,7 @@ def check_device_errors() -> None:
         raise KernelError(lib.mllm_last_error().decode(errors="replace"))
     if code.value:
         raise KernelError(f"the tree attention gave up waiting: code {code.value} "
-                          "(1-6 the issuing warps, 7-10 the softmax warps, 11 shared memory is not aligned)")
+                          "(1-6 the issuing warps, 7-10 the softmax warps, 11 and 22 shared memory that is not aligned, 21 a tile of keys or values)")
 
 
 class _Scope(threading.local):
@@ -2365,16 +2360,27 @@ def _attend(impl, q, ldq, k_pages, v_pages, block_table, bt_stride, ctx, out, ld
 # DRAFT_MAX_NODES of them.  Row 0 of a request is the token that is decided already, every other row names the row of its own request
 # that it hangs on (parents: an earlier row; -1: on the text itself).  Lengths, trees and results are int32 tensors on the device, so
 # that a step can follow the one before it without the host knowing how many tokens that one kept.  A request may bring no row.
+# Arguments go to C as one block of 64-bit fields (csrc/draft.cu): converted one by one they would take longer than the launch.
 DRAFT_MAX_NODES = 256
+_PACK_TABLES, _PACK_TREE, _PACK_ACCEPT, _PACK_KEEP = (struct.Struct(f) for f in ("15q", "29qd", "18q", "15q"))
 
 
-def _request_ints(who: str, lengths, cu_nodes) -> int:
-    _cuda("lengths", lengths, torch.int32)
-    _cuda("cu_nodes", cu_nodes, torch.int32)
-    S = lengths.numel()
+def _i32(name: str, t) -> int:
+    """The address of a contiguous int32 CUDA tensor."""
+    try:
+        if t.dtype is torch.int32 and t.is_cuda and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    return _cuda(name, t, torch.int32).data_ptr()          # raises
+
+
+def _requests(who: str, lengths, cu_nodes):
+    """(requests, address of lengths, address of cu_nodes)"""
+    pl, pc, S = _i32("lengths", lengths), _i32("cu_nodes", cu_nodes), lengths.numel()
     if cu_nodes.numel() != S + 1:
         raise KernelError(f"{who}: {S} requests need {S + 1} starts of their rows, got {cu_nodes.numel()}")
-    return S
+    return S, pl, pc
 
 
 def draft_tables(lengths, cu_nodes, parents, pages, cu_pages, page_size: int, *, block_table, slot_mapping, positions, token_seq,
@@ -2388,55 +2394,82 @@ def draft_tables(lengths, cu_nodes, parents, pages, cu_pages, page_size: int, *,
     length + i; -1, stored nowhere, where the request holds no page for it), ``positions`` [T] (length + depth in the
     tree), ``token_seq`` [T], ``ctx_len`` [S] (length + rows) and ``ancestors`` [T, words]: bit b of word w says that row
     32 w + b of the request is the row itself or on its way to the root.  Rows past 32 * words take no part: no slot, no bits."""
-    S = _request_ints("draft_tables", lengths, cu_nodes)
-    for name, t in (("pages", pages), ("cu_pages", cu_pages), ("block_table", block_table), ("slot_mapping", slot_mapping),
-                    ("positions", positions), ("token_seq", token_seq), ("ctx_len", ctx_len)):
-        _cuda(name, t, torch.int32)
+    S, p_len, p_cu = _requests("draft_tables", lengths, cu_nodes)
+    p_pages, p_cp, p_bt, p_slot, p_pos, p_seq, p_ctx = (
+        _i32("pages", pages), _i32("cu_pages", cu_pages), _i32("block_table", block_table), _i32("slot_mapping", slot_mapping),
+        _i32("positions", positions), _i32("token_seq", token_seq), _i32("ctx_len", ctx_len))
     T = slot_mapping.numel()
-    if block_table.dim() != 2 or block_table.shape[0] != S or cu_pages.numel() != S + 1 or ctx_len.numel() != S \
-            or positions.numel() != T or token_seq.numel() != T:
+    if block_table.dim() != 2 or cu_pages.numel() != S + 1 or ctx_len.numel() != S or positions.numel() != T or token_seq.numel() != T \
+            or block_table.shape[0] != S:
         raise KernelError(f"draft_tables: the tables of {S} requests and {T} rows do not fit: block_table {tuple(block_table.shape)}, "
                           f"cu_pages {cu_pages.numel()}, ctx_len {ctx_len.numel()}, positions {positions.numel()}, "
                           f"token_seq {token_seq.numel()}")
-    words = 0
+    words = p_anc = p_par = 0
     if ancestors is not None:
-        _cuda("ancestors", ancestors, torch.int32)
+        p_anc = _i32("ancestors", ancestors)
         if ancestors.dim() != 2 or ancestors.shape[0] != T or not 1 <= ancestors.shape[1] <= DRAFT_MAX_NODES // 32:
             raise KernelError(f"draft_tables: ancestors must be [{T}, 1 to {DRAFT_MAX_NODES // 32}], got {tuple(ancestors.shape)}")
         words = ancestors.shape[1]
     if parents is not None:
-        _cuda("parents", parents, torch.int32)
+        p_par = _i32("parents", parents)
         if parents.numel() != T or ancestors is None:
             raise KernelError(f"draft_tables: a tree needs a parent for each of its {T} rows, and ancestors to write")
     if page_size <= 0:
         raise KernelError(f"draft_tables: pages of {page_size} tokens")
-    _call("mllm_draft_tables", lengths.data_ptr(), cu_nodes.data_ptr(), None if parents is None else parents.data_ptr(),
-          pages.data_ptr(), cu_pages.data_ptr(), S, int(page_size), block_table.data_ptr(), block_table.shape[1],
-          slot_mapping.data_ptr(), positions.data_ptr(), token_seq.data_ptr(), ctx_len.data_ptr(),
-          None if ancestors is None else ancestors.data_ptr(), words, _stream())
+    _call("mllm_draft_tables", _PACK_TABLES.pack(p_len, p_cu, p_par, p_pages, p_cp, p_bt, p_slot, p_pos, p_seq, p_ctx, p_anc, S, page_size,
+                                                 block_table.shape[1], words), _stream())
 
 
 TREE_UNIT = 64               # keys of a unit of work of a tree attention that is cut along its keys
-TREE_JOIN_KEYS = 512         # what joining the parts costs, in keys that a block could walk instead
+TREE_JOIN_ROUNDS = {True: 2, False: 4}      # what the parts' join and the changes between them cost, in rounds of a block (float32, bfloat16)
 
 
-@functools.lru_cache(maxsize=1024)
-def tree_plan(float32: bool, S: int, num_heads: int, num_kv_heads: int, head_dim: int, max_nodes: int, max_length: int, tcgen05: bool,
+@functools.lru_cache(maxsize=256)
+def _tree_variant(float32: bool, head_dim: int, tile: int, wide: int):
+    """(blocks that an SM holds, keys that a block walks at once), or None where there is no such kernel."""
+    info = (c_int * 2)()
+    rc = library().mllm_tree_attention_variant(head_dim, tile, wide, F32 if float32 else BF16, info)
+    return None if rc else (info[0], info[1])
+
+
+@functools.lru_cache(maxsize=4096)
+def tree_plan(float32: bool, S: int, num_heads: int, num_kv_heads: int, head_dim: int, max_nodes: int, max_length: int, boxes: bool,
               sms: int):
     """How a tree attention is cut: (query rows of a tile, those of the largest tree, blocks that share the keys evenly (0: one for
-    every pair of tile and key/value head), whether a pair's block is a wide one).  ``tcgen05``: the kernel on tensor memory takes
-    these heads and pages."""
+    every pair of tile and key/value head), units that a block takes at least, variant).  ``boxes``: pages come by TMA.
+
+    Tiles.  float32: the smallest of 4, 8 and 16 that holds a tree's rows of one key/value head (more rows are more tiles: keys and
+    values come from L2 again, which costs less than warps that wait for one another; 5 requests, up to 37 rows, 25 heads of 64:
+    166 us in tiles of 16, 257 in tiles of 64).  bfloat16: tiles of 16 on mma.sync while few are needed, tensor memory beyond
+    (32 rows, 8 requests, 12 heads of 64: 15.6 us in two tiles of 16, 16.9; 64 rows: 19.7 and 19.4; heads of 128, 32 over 8, 32 rows:
+    37.4 and 31.4), except for heads over 128 and pages that no box fits.
+
+    Blocks.  A round is what a block walks at once.  A block per pair takes as many as the longest request, times the waves of
+    pairs; sharing the keys out evenly takes their sum, and the join.  Variants differ in groups per block: 1, more groups for few
+    pairs, 2, fewer for many blocks.  12 pairs of 518 keys: 9.3 us in wide blocks, 10.7 in others, 13.4 shared; 192 pairs of up to
+    1,008: 15.3 in blocks of their own, 18.7 shared; 64 pairs of up to 8,004 (heads of 128): 103 and 41."""
     rows = max(1, max_nodes * (num_heads // num_kv_heads))
-    if tcgen05:
-        tile = 128 if rows <= 128 else 256
+    if float32:
+        tile = next((t for t in (4, 8) if rows <= t), 16)
+    elif boxes and head_dim <= 128:
+        tile = 16 if rows <= (32 if head_dim <= 64 else 16) else 128 if rows <= 128 else 256
     else:
-        tile = next((t for t in ((4, 8, 16, 32) if float32 else (16, 32)) if rows <= t), 64)
-    tiles = -(-rows // tile)
-    pairs, places = S * num_kv_heads * tiles, sms * library().mllm_tree_attention_per_sm(head_dim, tile, F32 if float32 else BF16)
-    keys = max_length + max_nodes
-    if -(-pairs // places) * keys <= pairs * keys // places + TREE_JOIN_KEYS:
-        return tile, rows, 0, pairs <= sms
-    return tile, rows, places, False
+        tile = 16 if rows <= 16 else 32 if rows <= 64 or head_dim > 128 else 64
+    pairs, keys, best = S * num_kv_heads * -(-rows // tile), max_length + max_nodes, None
+    for wide in (0, 1, 2):
+        v = _tree_variant(float32, head_dim, tile, wide)
+        if v is None:
+            continue
+        places, at_once = v[0] * sms, v[1]
+        own = -(-pairs // places) * -(-keys // at_once)
+        shared = -(-pairs * keys // (places * at_once))
+        if best is None or own < best[0]:
+            best = own, (tile, rows, 0, 1, wide)
+        if wide == 0 or (wide == 2 and shared >= 8 and head_dim <= 64):
+            cost = shared + TREE_JOIN_ROUNDS[float32] - (0.5 if wide == 2 else 0)
+            if cost < best[0]:
+                best = cost, (tile, rows, places, max(1, at_once // TREE_UNIT), wide)
+    return best[1]
 
 
 def tree_attention(q, k_pages, v_pages, block_table, lengths, cu_nodes, ancestors, out, *, num_heads, num_kv_heads, head_dim, scale,
@@ -2449,45 +2482,53 @@ def tree_attention(q, k_pages, v_pages, block_table, lengths, cu_nodes, ancestor
     block_table [S, width].  ``max_nodes`` and ``max_length``: the most rows and the longest text that a request brings, where the
     host knows them; they only decide how the work is cut (without them: what ancestors and block_table can hold)."""
     global launches
-    S = _request_ints("tree_attention", lengths, cu_nodes)
+    S, p_len, p_cu = _requests("tree_attention", lengths, cu_nodes)
+    p_anc = _i32("ancestors", ancestors)
     _cuda("q", q, contiguous=False)
-    _cuda("k_pages", k_pages, q.dtype)
-    _cuda("v_pages", v_pages, q.dtype)
-    _cuda("out", out, q.dtype, contiguous=False)
+    dtype = q.dtype
+    _cuda("k_pages", k_pages, dtype)
+    _cuda("v_pages", v_pages, dtype)
+    _cuda("out", out, dtype, contiguous=False)
     _cuda("block_table", block_table, torch.int32, contiguous=False)
-    _cuda("ancestors", ancestors, torch.int32)
-    ldq, ldo, bt_stride = _rows("q", q), _rows("out", out), _rows("block_table", block_table)
-    T, dt = q.shape[0], _dt(q)
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
-        raise KernelError(f"tree_attention: pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    P, Hkv, ps, dh = k_pages.shape
-    if Hkv != num_kv_heads or dh != head_dim or q.shape[1] != num_heads * head_dim or tuple(out.shape) != tuple(q.shape) \
-            or num_heads % num_kv_heads:
+    ldq, ldo, bt_stride, dt = _rows("q", q), _rows("out", out), _rows("block_table", block_table), _dt(q)
+    shape = k_pages.shape
+    if len(shape) != 4 or shape != v_pages.shape:
+        raise KernelError(f"tree_attention: pages {tuple(shape)} and {tuple(v_pages.shape)}")
+    P, Hkv, ps, dh = shape
+    T, cols = q.shape
+    if Hkv != num_kv_heads or dh != head_dim or cols != num_heads * head_dim or out.shape != q.shape or num_heads % num_kv_heads:
         raise KernelError("tree_attention: head counts or sizes do not fit the pages")
     if head_dim % 16 != 0 or not (16 <= head_dim <= 256):
         raise KernelError(f"tree_attention: head size {head_dim} is not a multiple of 16 in 16..256")
-    if block_table.shape[0] != S:
+    n_tables, width = block_table.shape
+    if n_tables != S:
         raise KernelError(f"tree_attention: block_table {tuple(block_table.shape)} for {S} requests")
     if ancestors.dim() != 2 or ancestors.shape[0] != T or not 1 <= ancestors.shape[1] <= DRAFT_MAX_NODES // 32:
         raise KernelError(f"tree_attention: ancestors must be [{T}, 1 to {DRAFT_MAX_NODES // 32}], got {tuple(ancestors.shape)}")
     if T == 0 or S == 0:
         return
-    width, words = block_table.shape[1], ancestors.shape[1]
-    tile, rows, blocks, wide = tree_plan(
+    words = ancestors.shape[1]
+    tile, rows, blocks, least, wide = tree_plan(
         dt == F32, S, num_heads, num_kv_heads, head_dim, min(T, 32 * words if max_nodes is None else int(max_nodes)),
-        width * ps if max_length is None else min(int(max_length), width * ps),
-        dt == BF16 and use_tcgen05_attention and head_dim <= 128 and ps % 8 == 0, sm_count())
-    part_o = part_ml = None
+        width * ps if max_length is None else min(int(max_length), width * ps), ps % 8 == 0, sm_count())
+    part_o = part_ml = cuts = 0
     if blocks:
         parts = 2 * blocks * tile
-        part_o = _scratch("tree_attn", q.device, parts * (head_dim + 2)).data_ptr()
+        cuts = _scratch("tree_attn", q.device, parts * (head_dim + 2) + 8 * blocks).data_ptr()
+        part_o = cuts + 32 * blocks
         part_ml = part_o + 4 * parts * head_dim
     attention_launches["tree"] = attention_launches.get("tree", 0) + 1
-    _call("mllm_tree_attention", q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), P, block_table.data_ptr(), bt_stride, width,
-          lengths.data_ptr(), cu_nodes.data_ptr(), ancestors.data_ptr(), words, out.data_ptr(), ldo, part_o, part_ml, S, num_heads,
-          num_kv_heads, head_dim, ps, float(scale), tile, rows, TREE_UNIT, blocks, wide, dt, _stream())
+    _call("mllm_tree_attention", _PACK_TREE.pack(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), p_len, p_cu, p_anc, out.data_ptr(), part_o, part_ml, cuts,
+        ldq, ldo, P, bt_stride, width, words, S, num_heads, num_kv_heads, head_dim, ps, tile, rows, TREE_UNIT, least, blocks, wide, dt, scale),
+        _stream())
     if blocks:
         launches += 1           # the kernel in which the parts meet
+
+
+def accept_slices(rows: int, vocab: int) -> int:
+    """Slices into which each of ``rows`` rows of logits is cut: enough blocks for every SM (32 each), none under 2,048 logits."""
+    return max(1, min(-(-4736 // max(rows, 1)), -(-vocab // 2048)))
 
 
 def accept_drafts(tokens, parents, cu_nodes, lengths, *, chosen, path, accepted, next_token, new_lengths, logits=None) -> None:
@@ -2501,18 +2542,17 @@ def accept_drafts(tokens, parents, cu_nodes, lengths, *, chosen, path, accepted,
     ``new_lengths`` [S] (lengths + accepted; may be ``lengths`` itself).  Trees have at most DRAFT_MAX_NODES rows; rows past
     that are on no path."""
     global launches
-    S = _request_ints("accept_drafts", lengths, cu_nodes)
-    for name, t in (("tokens", tokens), ("parents", parents), ("chosen", chosen), ("path", path), ("accepted", accepted),
-                    ("next_token", next_token), ("new_lengths", new_lengths)):
-        _cuda(name, t, torch.int32)
+    S, p_len, p_cu = _requests("accept_drafts", lengths, cu_nodes)
+    p_tok, p_par, p_cho, p_path, p_acc, p_next, p_new = (
+        _i32("tokens", tokens), _i32("parents", parents), _i32("chosen", chosen), _i32("path", path), _i32("accepted", accepted),
+        _i32("next_token", next_token), _i32("new_lengths", new_lengths))
     T = tokens.numel()
     if parents.numel() != T or chosen.numel() != T or path.dim() != 2 or path.shape[0] != S or path.shape[1] < 1 \
             or accepted.numel() != S or next_token.numel() != S or new_lengths.numel() != S:
         raise KernelError(f"accept_drafts: arguments for {S} requests and {T} rows do not fit: parents {parents.numel()}, chosen "
                           f"{chosen.numel()}, path {tuple(path.shape)}, accepted {accepted.numel()}, next_token "
                           f"{next_token.numel()}, new_lengths {new_lengths.numel()}")
-    ld = V = slices = 0
-    part_val = part_idx = None
+    ld = V = slices = p_logits = part_val = part_idx = 0
     if logits is not None:
         _cuda("logits", logits, torch.float32, contiguous=False)
         ld = _rows("logits", logits)
@@ -2520,12 +2560,12 @@ def accept_drafts(tokens, parents, cu_nodes, lengths, *, chosen, path, accepted,
         if logits.shape[0] != T or V < 1:
             raise KernelError(f"accept_drafts: logits {tuple(logits.shape)} for {T} rows")
         if T:
-            slices = library().mllm_accept_slices(T, V)
-            part_val = _scratch("accept", logits.device, 2 * T * slices).data_ptr()
+            p_logits, slices = logits.data_ptr(), accept_slices(T, V)
+            part = _scratch("accept", logits.device, 2 * T * slices)
+            part_val = part.data_ptr()
             part_idx = part_val + 4 * T * slices
-    _call("mllm_accept_drafts", None if logits is None else logits.data_ptr(), ld, T, V, slices, part_val, part_idx, chosen.data_ptr(),
-          tokens.data_ptr(), parents.data_ptr(), cu_nodes.data_ptr(), lengths.data_ptr(), S, path.data_ptr(), path.shape[1],
-          accepted.data_ptr(), next_token.data_ptr(), new_lengths.data_ptr(), _stream())
+    _call("mllm_accept_drafts", _PACK_ACCEPT.pack(p_logits, part_val, part_idx, p_cho, p_tok, p_par, p_cu, p_len, p_path, p_acc, p_next, p_new,
+                                                  ld, T, V, slices, S, path.shape[1]), _stream())
     if slices:
         launches += 1           # the kernel that reads the logits
 
@@ -2536,8 +2576,7 @@ def keep_accepted(planes, block_table, lengths, path, accepted) -> None:
     ``planes`` [..., num_pages, heads, page_size, d]: a cache group's pool, or its keys and values one after the other."""
     _cuda("planes", planes)
     _cuda("block_table", block_table, torch.int32, contiguous=False)
-    for name, t in (("lengths", lengths), ("path", path), ("accepted", accepted)):
-        _cuda(name, t, torch.int32)
+    p_len, p_path, p_acc = _i32("lengths", lengths), _i32("path", path), _i32("accepted", accepted)
     S = lengths.numel()
     bt_stride = _rows("block_table", block_table)
     if planes.dim() < 4 or path.dim() != 2 or path.shape[0] != S or path.shape[1] < 1 or accepted.numel() != S \
@@ -2549,8 +2588,9 @@ def keep_accepted(planes, block_table, lengths, path, accepted) -> None:
     plane = P * heads * ps * d
     if plane == 0:
         return
-    _call("mllm_keep_accepted", planes.data_ptr(), plane * es, planes.numel() // plane, P, heads, ps, d * es, block_table.data_ptr(),
-          bt_stride, block_table.shape[1], lengths.data_ptr(), path.data_ptr(), path.shape[1], accepted.data_ptr(), S, _stream())
+    _call("mllm_keep_accepted", _PACK_KEEP.pack(planes.data_ptr(), block_table.data_ptr(), p_len, p_path, p_acc, plane * es,
+                                                planes.numel() // plane, P, heads, ps, d * es, bt_stride, block_table.shape[1],
+                                                path.shape[1], S), _stream())
 
 
 # --------------------------------------------------------------------------- sampling
