@@ -431,7 +431,10 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
             }
             done += max(steps, 1);
             if (alive) {
-                bool got = mbar_wait(&bars.o_full[x], (done - 1) & 1);
+                // the last product, and with two sets of scores the one before it first: that may not be complete either, and a wait
+                // for a phase two ahead of the barrier's own looks like one for the phase behind it
+                bool got = SB == 1 || steps < 2 || mbar_wait(&bars.o_full[x], (done - 2) & 1);
+                got = got && mbar_wait(&bars.o_full[x], (done - 1) & 1);
                 if (!got) *failed = 8;
                 alive = __all_sync(0xffffffffu, got && !*failed);
             }

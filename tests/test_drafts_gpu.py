@@ -218,6 +218,21 @@ def test_attention_over_spans(ops, dtype, S, length):
     Case(dtype, [length - 7 * s for s in range(S)], [8] * S, 4, 2, 64, 16, seed=S).check(ops)
 
 
+@pytest.mark.parametrize("dtype,lengths,n,H,Hkv,d,ps", [
+    (torch.bfloat16, [6001, 3000, 9], 40, 8, 2, 128, 64), (torch.bfloat16, [2500, 6001], 20, 8, 2, 128, 16),
+    (torch.bfloat16, [5000, 64], 48, 3, 1, 64, 16), (torch.bfloat16, [4000, 700], 100, 6, 2, 64, 8), (torch.bfloat16, [7000], 70, 8, 1, 80, 32),
+    (torch.float32, [3000, 1, 900], 20, 4, 2, 128, 16), (torch.bfloat16, [3000, 1, 900], 70, 4, 2, 64, 5)])
+def test_long_texts_and_wide_trees(ops, dtype, lengths, n, H, Hkv, d, ps):
+    """Keys shared out among blocks, in every kernel that takes many rows: several segments a block, values that come late."""
+    counts = [n, max(1, n // 2), 3][:len(lengths)]
+    c = Case(dtype, lengths, counts, H, Hkv, d, ps, seed=n + d)
+    filler = torch.randn(1 << 27, device=DEV)             # more than L2: keys and values come from memory
+    for _ in range(3):
+        filler.mul_(1.0)
+        c.out.fill_(7.0)
+        c.check(ops)
+
+
 @pytest.mark.parametrize("dtype", BOTH)
 def test_hints_only_change_how_the_work_is_cut(ops, dtype):
     for hints in (dict(), dict(max_nodes=20, max_length=700), dict(max_nodes=1, max_length=1), dict(max_nodes=256, max_length=100000)):
