@@ -21,10 +21,13 @@ def __getattr__(name):
     if name == "LLM":          # needs CUDA at construction only; imported on demand
         from .engine.llm import LLM
         return LLM
+    if name == "PromptLookup":
+        from .engine.drafting import PromptLookup
+        return PromptLookup
     raise AttributeError(name)
 
 
 __all__ = ["ConfigError", "EngineConfig", "config_from_dict", "load_config", "register_architecture",
            "registered_architectures", "register_part", "write_random_model", "SamplingParams", "Request",
-           "RequestState", "Response", "LLM"]
+           "RequestState", "Response", "LLM", "PromptLookup"]
 __version__ = "0.1.0"

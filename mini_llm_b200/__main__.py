@@ -50,6 +50,9 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--ignore-eos", action="store_true")
     ap.add_argument("--prompt-ids", action="append", default=[], help='one request, e.g. "15496 11 616 1438 318"')
     ap.add_argument("--prompts-file", help="one request per line of token ids ('-' = standard input)")
+    ap.add_argument("--draft-rows", type=int, default=0, metavar="N",
+                    help="check N rows per request and pass: its last token and guesses taken from its own text (0 = off)")
+    ap.add_argument("--draft-depth", type=int, default=8, help="with --draft-rows: tokens that a pass keeps at most")
     ap.add_argument("--stream", action="store_true", help="print every token as it is produced: '<request> <id>'")
     ap.add_argument("--stats", action="store_true", help="print scheduler counters to standard error")
     ap.add_argument("--metrics", action="store_true",
@@ -99,6 +102,17 @@ def main(argv=None) -> int:
         llm.profile = []
     sp = SamplingParams(temperature=args.temperature, seed=args.sample_seed, max_new_tokens=args.max_new_tokens,
                         ignore_eos=args.ignore_eos)
+    if args.draft_rows:
+        if args.stream or args.metrics or args.profile:
+            print("--draft-rows cannot be combined with --stream, --metrics or --profile", file=sys.stderr)
+            return 1
+        for out in llm.generate_drafted(prompts, sp, rows=args.draft_rows, depth=min(args.draft_depth, args.draft_rows)):
+            print(" ".join(str(t) for t in out) + " [DONE]")
+        if args.stats:
+            print(json.dumps(vars(llm.draft_stats)), file=sys.stderr)
+        if tmp is not None:
+            tmp.cleanup()
+        return 0
     ids = [llm.add_request(p, sp) for p in prompts]
     outs = {i: [] for i in ids}
     while llm.has_unfinished():

@@ -32,6 +32,18 @@ class GroupView:
 
 
 @dataclass
+class TreeView:
+    """A step of trees of drafted tokens: row i of request s is the step's token cu_nodes[s] + i and sees the request's first
+    lengths[s] cached tokens and the rows of its own tree whose bit is set."""
+
+    lengths: torch.Tensor          # int32 [S]
+    cu_nodes: torch.Tensor         # int32 [S + 1]
+    ancestors: torch.Tensor        # int32 [T, words]
+    max_nodes: int
+    max_length: int
+
+
+@dataclass
 class StepLayout:
     """Offsets (in int32 elements) of every section of the packed buffer."""
 
@@ -127,6 +139,8 @@ class Workspace:
 
 class StepContext:
     """Device views of one step's packed integers, plus host-side facts about it."""
+
+    tree: Optional[TreeView] = None      # set in steps of drafted tokens (engine/drafting.py)
 
     def __init__(self, layout: StepLayout, dev: torch.Tensor, ws: Workspace, *, q_lens: Sequence[int],
                  q_starts: Sequence[int]):

@@ -1,0 +1,390 @@
+"""Decoding with drafted tokens: several guesses per request are checked in one pass of the model.
+
+A decode step of a few requests takes as long as reading the weights takes, however few tokens it computes.  So a request
+may bring, beside its last token, a tree of guesses of what follows (``PromptLookup`` takes them from the request's own
+text); one pass gives the model's own choice behind every row of the tree, and the longest path that agrees with those
+choices is kept: the same tokens as without drafts (where two logits are closer than the kernels' rounding, either), one
+to ``depth`` of them per pass.  Sampling with a temperature draws each row's choice with the uniform number that belongs to
+that token's place, so it gives the tokens that it would have drawn one at a time.
+
+The device does what lies between two passes: ``ops.draft_tables`` (cache slots, positions and visibility bits from lengths
+and page lists), ``ops.tree_attention``, ``ops.accept_drafts``, ``ops.keep_accepted``.
+
+The reference decodes one token per request and call (src/model/gpt2_model.cu:455-689) and has no counterpart.
+"""
+from __future__ import annotations
+
+from collections import deque
+from dataclasses import dataclass, field
+from typing import Dict, Hashable, List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from .. import ops
+from ..sampling.params import SamplingParams, uniform_for
+from .context import GroupView, TreeView
+from .request import Request
+from .runner import ModelRunner, OutOfPages, StepEntry, StepError
+
+
+class PromptLookup:
+    """Guesses that what followed the last few tokens earlier in the text follows them again.
+
+    The longest suffix of up to ``ngram`` tokens that occurs earlier decides, then shorter ones while there is room; the most
+    recent of up to ``branches`` occurrences come first.  Continuations that begin alike share rows."""
+
+    def __init__(self, ngram: int = 3, branches: int = 4):
+        if ngram < 1 or branches < 1:
+            raise ValueError("PromptLookup: ngram and branches must be at least 1")
+        self.ngram, self.branches = int(ngram), int(branches)
+
+    def draft(self, tokens: Sequence[int], rows: int, depth: int) -> Tuple[List[int], List[int]]:
+        """(tokens, parents) of a tree of at most ``rows`` rows and ``depth`` rows from its root, the last token."""
+        text = np.asarray(tokens, dtype=np.int64)
+        out, parents = [int(text[-1])], [-1]
+        child: Dict[Tuple[int, int], int] = {}
+        left, n = self.branches, min(self.ngram, len(text) - 1)
+        ends: set = set()
+        while n >= 1 and left > 0 and depth > 1 and len(out) < rows:
+            hit = np.ones(len(text) - n, dtype=bool)          # does the suffix end before place i + n?
+            for k in range(n):
+                hit &= text[k:k + len(hit)] == text[len(text) - n + k]
+            for end in (np.nonzero(hit)[0][::-1] + n).tolist():
+                if left == 0 or len(out) >= rows:
+                    break
+                if end in ends:
+                    continue
+                ends.add(end)
+                left -= 1
+                at = 0
+                for tok in text[end:end + depth - 1].tolist():
+                    nxt = child.get((at, tok))
+                    if nxt is None:
+                        if len(out) >= rows:
+                            break
+                        nxt = child[(at, tok)] = len(out)
+                        out.append(tok)
+                        parents.append(at)
+                    at = nxt
+            n -= 1
+        return out, parents
+
+
+@dataclass
+class DraftEntry:
+    """One request's tree: row 0 is its last token (not in the cache yet), row i hangs on row ``parents[i]`` < i; a row that hangs on
+    none (-1) is on no path.  ``uniform``: a number in [0, 1) per row, where the temperature is not 0."""
+
+    req: Hashable
+    tokens: Sequence[int]
+    parents: Sequence[int]
+    temperature: float = 0.0
+    uniform: Sequence[float] = ()
+
+
+@dataclass
+class DraftResult:
+    tokens: List[int]          # new tokens: the drafted ones that were right, then the model's own
+    rows: List[int]            # the path: rows of the tree that the cache now holds
+
+
+@dataclass
+class DraftStats:
+    steps: int = 0
+    requests: int = 0          # trees checked
+    tokens: int = 0            # tokens that came of them
+
+
+class _TreeLayout:
+    def __init__(self, T: int, S: int, max_pages: Tuple[int, ...], words: int, rows: int):
+        self._key = (T, S, T, max_pages, "tree", words, rows)
+
+    def key(self):
+        return self._key
+
+
+class DraftContext:
+    """What the parts of a model see of a step of trees: a ``StepContext`` with a ``tree`` (and no tiles of prompt portions)."""
+
+    n_tiles = n_tiles_wide = 0
+    attn_tiles = attn_tiles_wide = None
+    single_runs: tuple = ()
+    decode_only = False
+    max_single_ctx_len = 0
+
+    def __init__(self, **facts):
+        self.carry = None
+        self.__dict__.update(facts)
+
+
+class DraftRunner:
+    """Steps of trees on a ``ModelRunner``: ``rows`` per request and step at most, paths of up to ``depth`` rows."""
+
+    def __init__(self, runner: ModelRunner, rows: int = 16, depth: int = 8):
+        if not 1 <= depth <= rows <= ops.DRAFT_MAX_NODES:
+            raise ValueError(f"drafts: 1 <= depth <= rows <= {ops.DRAFT_MAX_NODES}, got depth {depth} and {rows} rows")
+        cannot = sorted({type(l.mixer).__name__ for l in runner.model.layers if not getattr(l.mixer, "takes_trees", False)})
+        windows = [g for g in runner.cache.groups if g.need.window is not None or g.need.chunk is not None]
+        if cannot or windows or runner.cache.state_layers:
+            raise StepError("drafts need layers whose attention sees all of the text and that carry no state from token to token; "
+                            f"this model has {', '.join(cannot) or 'a window or a state'}")
+        self.runner, self.rows, self.depth = runner, int(rows), int(depth)
+        self.words = -(-self.rows // 32)
+        self._host: List[Optional[torch.Tensor]] = [None, None]
+        self._dev: Optional[torch.Tensor] = None
+
+    def _ints(self, n: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(pinned host buffer, device buffer) of at least n 32-bit words; captured graphs are dropped when the latter moves."""
+        if self._dev is None or self._dev.numel() < n:
+            cap = max(1 << 14, 1 << (n - 1).bit_length())
+            self._host = [torch.empty(cap, dtype=torch.int32, pin_memory=True) for _ in range(2)]
+            self._dev = torch.zeros(cap, dtype=torch.int32, device=self.runner.device)
+            self.runner.ws.version += 1
+        return self._host[0], self._dev
+
+    def step(self, entries: Sequence[DraftEntry]) -> List[DraftResult]:
+        """One pass over all trees; the accepted rows' keys and values are in the cache afterwards, and committed."""
+        r, cm, R = self.runner, self.runner.cache, self.rows
+        S = len(entries)
+        if S == 0:
+            raise StepError("a step needs at least one entry")
+        if len({e.req for e in entries}) != S:
+            raise StepError("a request appears twice in one step")
+        T, ng, depth = S * R, len(cm.groups), self.depth
+        tokens, parents = np.zeros((S, R), np.int32), np.full((S, R), -1, np.int32)
+        deepest = 0
+        for s, e in enumerate(entries):
+            n = len(e.tokens)
+            if not cm.is_live(e.req):
+                raise StepError(f"request {e.req!r} is not live (add_request first)")
+            if not 1 <= n <= R or len(e.parents) != n:
+                raise StepError(f"request {e.req!r}: a tree of {n} rows and {len(e.parents)} parents; 1 to {R} rows are taken")
+            if e.temperature > 0 and len(e.uniform) != n:
+                raise StepError(f"request {e.req!r}: a temperature needs a uniform number for each of {n} rows")
+            if any(not 0 <= int(t) < r.vocab_size for t in e.tokens):
+                raise StepError(f"request {e.req!r}: a token id is outside the vocabulary of {r.vocab_size}")
+            level = [0] * n
+            for i, p in enumerate(e.parents):
+                if not -1 <= p < i:
+                    raise StepError(f"request {e.req!r}: row {i} hangs on row {p}, which does not come before it")
+                level[i] = level[p] + 1 if p >= 0 else 0
+            start = cm.computed(e.req)
+            if r.max_positions is not None and start + max(level) >= r.max_positions:
+                raise StepError(f"request {e.req!r}: {start + max(level) + 1} tokens exceed the model's {r.max_positions} positions")
+            tokens[s, :n], parents[s, :n] = e.tokens, e.parents
+            deepest = max(deepest, start)
+        for e in entries:
+            if not cm.reserve(e.req, R):
+                raise OutOfPages(f"no pages left for {R} rows of request {e.req!r}")
+        lists = [[cm.table(e.req, g) for e in entries] for g in range(ng)]
+        widths = tuple(max(16, 1 << (max(len(t) for t in lists[g]) - 1).bit_length()) for g in range(ng))
+        sampled = any(e.temperature > 0 for e in entries)
+
+        # one packed buffer: what the host sends, then what the device makes and returns
+        at: Dict[str, Tuple[int, int]] = {}
+        end = 0
+
+        def section(name, n):
+            nonlocal end
+            at[name] = (end, n)
+            end += (n + 3) & ~3
+
+        for name, n in (("tokens", T), ("parents", T), ("rows", T), ("lengths", S), ("cu", S + 1), ("temperature", T), ("uniform", T),
+                        ("positions", T), ("seq", T), ("ctx_len", S), ("ancestors", T * self.words), ("chosen", T), ("path", S * depth),
+                        ("accepted", S), ("next", S), ("new_lengths", S)):
+            section(name, n)
+        for g in range(ng):
+            section(f"slots.{g}", T)
+            section(f"table.{g}", S * widths[g])
+        for g in range(ng):                              # the page lists last: their sizes change from step to step
+            section(f"cu_pages.{g}", S + 1)
+            section(f"pages.{g}", sum(len(t) for t in lists[g]))
+        host, dev = self._ints(end)
+        h = host.numpy()
+
+        def put(name, values):
+            a, n = at[name]
+            h[a:a + n] = np.asarray(values).reshape(-1)
+
+        put("tokens", tokens)
+        put("parents", parents)
+        put("rows", np.arange(T, dtype=np.int32))
+        put("lengths", [cm.computed(e.req) for e in entries])
+        put("cu", np.arange(S + 1, dtype=np.int32) * R)
+        if sampled:
+            heat, uniform = np.zeros((S, R), np.float32), np.zeros((S, R), np.float32)
+            for s, e in enumerate(entries):
+                heat[s] = e.temperature
+                uniform[s, :len(e.uniform)] = e.uniform
+            put("temperature", heat.view(np.int32))
+            put("uniform", uniform.view(np.int32))
+        sent = at["positions"][0]
+        for g in range(ng):
+            put(f"cu_pages.{g}", np.concatenate([[0], np.cumsum([len(t) for t in lists[g]])]))
+            put(f"pages.{g}", np.concatenate([np.asarray(t, dtype=np.int32) for t in lists[g]]))
+        tail = at[f"cu_pages.0"][0]
+        dev[:sent].copy_(host[:sent], non_blocking=True)
+        dev[tail:end].copy_(host[tail:end], non_blocking=True)
+
+        def view(name, *shape):
+            a, n = at[name]
+            t = dev[a:a + n]
+            return t.view(shape) if shape else t
+
+        lengths, cu, ancestors = view("lengths"), view("cu"), view("ancestors", T, self.words)
+        groups = []
+        for g in range(ng):
+            table = view(f"table.{g}", S, widths[g])
+            slots = view(f"slots.{g}")
+            ops.draft_tables(lengths, cu, view("parents"), view(f"pages.{g}"), view(f"cu_pages.{g}"), cm.page_size, block_table=table,
+                             slot_mapping=slots, positions=view("positions"), token_seq=view("seq"), ctx_len=view("ctx_len"),
+                             ancestors=ancestors)
+            groups.append(GroupView(block_table=table, slot_mapping=slots, max_pages=widths[g]))
+        ctx = DraftContext(T=T, S=S, R=T, ws=r.ws, token_ids=view("tokens"), positions=view("positions"), token_seq=view("seq"),
+                           logit_rows=view("rows"), state_slots=None, q_start=lengths, ctx_len=view("ctx_len"), cu_q=cu, groups=groups,
+                           layout=_TreeLayout(T, S, widths, self.words, R), max_q_len=R, max_ctx_len=deepest + R,
+                           q_lens=[R] * S, q_starts=[cm.computed(e.req) for e in entries],
+                           tree=TreeView(lengths=lengths, cu_nodes=cu, ancestors=ancestors, max_nodes=R,
+                                         max_length=ops.split_context(deepest + R)))
+        logits = r._forward(ctx)
+        chosen, path, accepted, nxt = view("chosen"), view("path", S, depth), view("accepted"), view("next")
+        with ops.stream_scope(r.ws):
+            if sampled:
+                ops.sample(logits, view("temperature").view(torch.float32), view("uniform").view(torch.float32), chosen)
+            ops.accept_drafts(view("tokens"), view("parents"), cu, lengths, chosen=chosen, path=path, accepted=accepted, next_token=nxt,
+                              new_lengths=view("new_lengths"), logits=None if sampled else logits)
+            for g, gv in zip(cm.groups, groups):
+                for planes in ((g.pool,) if g.pool is not None else (g.pool_k, g.pool_v)):
+                    if planes is not None:
+                        ops.keep_accepted(planes, gv.block_table, lengths, path, accepted)
+        first, last = at["path"][0], at["new_lengths"][0]
+        back = self._host[1][:last - first]
+        back.copy_(dev[first:last], non_blocking=True)
+        torch.cuda.current_stream().synchronize()
+        ops.raise_if_kernel_gave_up()
+        r.steps_run += 1
+        b = back.numpy()
+        out = []
+        for s, e in enumerate(entries):
+            n = int(b[at["accepted"][0] - first + s])
+            rows = b[s * depth:s * depth + n].tolist()
+            cm.commit(e.req, n)
+            out.append(DraftResult([int(e.tokens[i]) for i in rows[1:]] + [int(b[at["next"][0] - first + s])], rows))
+        return out
+
+
+class DraftedDecoder:
+    """Generates for a list of requests with drafts: prompts in portions, then steps of trees.  Pages are taken for a request's
+    whole length when it starts; requests that find none wait."""
+
+    def __init__(self, llm, drafter=None, rows: int = 16, depth: int = 8):
+        self.llm, self.runner, self.drafter = llm, llm.runner, drafter if drafter is not None else PromptLookup()
+        self.trees = DraftRunner(llm.runner, rows, depth)
+        self.stats = DraftStats()
+
+    def _done(self, req: Request) -> bool:
+        limit = self.runner.max_positions
+        return req.ended_at is not None or req.isfinish() or (limit is not None and len(req.tokens) > limit)
+
+    def _take(self, req: Request, tokens: Sequence[int]) -> None:
+        eos = self.runner.spec.eos_token_id
+        for t in tokens:
+            if self._done(req):
+                return
+            if not req.params.ignore_eos and eos is not None and t == eos:
+                req.ended_at = len(req.tokens)
+            req.tokens.append(int(t))
+
+    def _start(self, waiting: deque, running: int) -> List[Request]:
+        cm, started = self.runner.cache, []
+        while waiting and cm.can_admit():
+            req = waiting[0]
+            total = len(req.tokens) + req.max_new_tokens
+            if self.runner.max_positions is not None:
+                total = min(total, self.runner.max_positions)
+            cm.admit(req.request_id)
+            if not cm.reserve(req.request_id, total + self.trees.rows):
+                cm.release(req.request_id)
+                if running + len(started) == 0:
+                    raise OutOfPages(f"request {req.request_id!r}: the cache has no pages for {total} tokens and {self.trees.rows} rows of drafts")
+                break
+            started.append(waiting.popleft())
+        return started
+
+    def _prompts(self, started: List[Request]) -> None:
+        """The prompts of new requests, in portions under the step's token budget; their first tokens."""
+        e, r = self.llm.engine_config, self.runner
+        left = deque(started)
+        while left:
+            entries, ready, budget = [], [], e.max_num_batched_tokens
+            for req in list(left):
+                n = min(len(req.tokens) - req.num_computed, e.prefill_chunk, budget)
+                if n <= 0:
+                    break
+                last = req.num_computed + n == len(req.tokens)
+                entries.append(StepEntry(req.request_id, req.portion(req.num_computed, req.num_computed + n), [n - 1] if last else []))
+                budget -= n
+                req.num_computed += n
+                if last:
+                    ready.append(req)
+                    left.remove(req)
+            logits = r.step(entries)
+            if ready:
+                for req, tok in zip(ready, self.llm.sampler.sample(logits, ready)):
+                    self._take(req, [tok])
+
+    def _tree(self, req: Request) -> DraftEntry:
+        depth = min(self.trees.depth, req.max_new_tokens - req.num_generated)
+        if self.runner.max_positions is not None:
+            depth = min(depth, self.runner.max_positions - self.runner.computed(req.request_id))
+        tokens, parents = self.drafter.draft(req.tokens, self.trees.rows, depth)
+        level = []
+        for p in parents:
+            level.append(0 if p < 0 else level[p] + 1)
+        sp = req.params
+        uniform = [uniform_for(sp.seed, req.request_id, req.num_generated + l) for l in level] if sp.temperature > 0 else ()
+        return DraftEntry(req.request_id, tokens, parents, sp.temperature, uniform)
+
+    def run(self, requests: Sequence[Request]) -> None:
+        """Until every request is done; ``request.tokens`` then ends with what was generated."""
+        waiting, live = deque(requests), []
+        at_once = max(1, self.llm.engine_config.max_num_batched_tokens // self.trees.rows)
+        try:
+            while waiting or live:
+                started = self._start(waiting, len(live))
+                self._prompts(started)
+                live += started
+                for first in range(0, len(live), at_once):
+                    batch = [q for q in live[first:first + at_once] if not self._done(q)]
+                    if not batch:
+                        continue
+                    for req, got in zip(batch, self.trees.step([self._tree(q) for q in batch])):
+                        before = len(req.tokens)
+                        self._take(req, got.tokens)
+                        self.stats.tokens += len(req.tokens) - before
+                    self.stats.steps += 1
+                    self.stats.requests += len(batch)
+                for req in [q for q in live if self._done(q)]:
+                    self.runner.finish_request(req.request_id)
+                    live.remove(req)
+        finally:
+            for req in requests:
+                if self.runner.has_request(req.request_id):
+                    self.runner.finish_request(req.request_id)
+
+
+def generate_drafted(llm, prompts: Sequence[Sequence[int]], params: Sequence[SamplingParams], drafter=None, rows: int = 16,
+                     depth: int = 8) -> Tuple[List[List[int]], DraftStats]:
+    decoder = DraftedDecoder(llm, drafter, rows, depth)
+    requests = []
+    limit = llm.runner.max_positions
+    for prompt, sp in zip(prompts, params):
+        if not prompt or any(not 0 <= int(t) < llm.runner.vocab_size for t in prompt):
+            raise ValueError("a prompt is empty, or a token id is outside the vocabulary")
+        if limit is not None and len(prompt) > limit:
+            raise ValueError(f"a prompt of {len(prompt)} tokens exceeds the model's {limit} positions")
+        requests.append(Request(llm._next_id, list(prompt), sp))
+        llm._next_id += 1
+    decoder.run(requests)
+    return [q.generated_tokens() for q in requests], decoder.stats

@@ -34,6 +34,7 @@ class LLM:
         self._inflight = None          # (advanced step, sampler ticket, request id -> row) of a step whose tokens are not read yet
         self._held: List[Response] = []     # responses read while aborting, handed out by the next step()
         self.metrics = ServingMetrics()      # arrival, first and last token of every request (host clock)
+        self.draft_stats = None              # of the last generate_drafted: passes, trees and the tokens that came of them
         self.profile = None                  # a list: step() then times every launch and appends a row per kernel
         self._profile_steps = 0
         self._last_step_shape = None
@@ -155,3 +156,23 @@ class LLM:
                 if resp.request_id in out:
                     out[resp.request_id].append(resp.token)
         return [out[i] for i in ids]
+
+    def generate_drafted(self, prompts: Sequence[Sequence[int]],
+                         sampling_params: Union[SamplingParams, Sequence[SamplingParams], None] = None, *, drafter=None,
+                         rows: int = 16, depth: int = 8) -> List[List[int]]:
+        """``generate`` with drafted tokens (engine/drafting.py): a pass of the model checks up to ``rows`` rows per request, the
+        last token and guesses of what follows it, and keeps up to ``depth`` tokens.  ``drafter``: an object with
+        ``draft(tokens, rows, depth) -> (tokens, parents)``; ``PromptLookup()`` where there is none.  For models whose layers
+        are attention over all of the text; refused for others, and while requests of ``add_request`` are unfinished.
+        ``draft_stats`` then says how many passes it took."""
+        from .drafting import generate_drafted
+        if self.has_unfinished():
+            raise RuntimeError("generate_drafted: requests of add_request are unfinished")
+        if sampling_params is None:
+            sampling_params = SamplingParams()
+        if isinstance(sampling_params, SamplingParams):
+            sampling_params = [sampling_params] * len(prompts)
+        if len(sampling_params) != len(prompts):
+            raise ValueError("one SamplingParams per prompt")
+        out, self.draft_stats = generate_drafted(self, prompts, sampling_params, drafter, rows, depth)
+        return out

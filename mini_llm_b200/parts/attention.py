@@ -26,6 +26,7 @@ from .projected import ProjectedMixer
 class Attention(Mixer):
     accepts_lazy_norm = True
     singles_apart = True         # in a step with prompt portions the single tokens take the decode kernel
+    takes_trees = True           # a step may bring trees of drafted tokens (without a window)
 
     def __init__(self, hidden_size: int, num_heads: int, head_dim: int, scale: float,
                  num_kv_heads: Optional[int] = None, window: Optional[int] = None, bias: bool = True):
@@ -84,9 +85,16 @@ class Attention(Mixer):
             if cache.write:
                 ops.kv_write(k, v, cache.k_pages, cache.v_pages, gv.slot_mapping)
         att = ctx.ws.buf("attn_out", T, self.q_size, self.rt.act_dtype)
-        ops.paged_attention(q, cache.k_pages, cache.v_pages, gv.block_table, ctx, att,
-                            num_heads=self.num_heads, num_kv_heads=self.num_kv_heads,
-                            head_dim=self.head_dim, scale=self.scale, window=self.window)
+        tree = getattr(ctx, "tree", None)
+        if tree is not None:
+            ops.tree_attention(q, cache.k_pages, cache.v_pages, gv.block_table, tree.lengths, tree.cu_nodes,
+                               tree.ancestors, att, num_heads=self.num_heads, num_kv_heads=self.num_kv_heads,
+                               head_dim=self.head_dim, scale=self.scale, max_nodes=tree.max_nodes,
+                               max_length=tree.max_length)
+        else:
+            ops.paged_attention(q, cache.k_pages, cache.v_pages, gv.block_table, ctx, att,
+                                num_heads=self.num_heads, num_kv_heads=self.num_kv_heads,
+                                head_dim=self.head_dim, scale=self.scale, window=self.window)
         ops.linear(att, self.out_weight, self.out_bias, out=out_accum, accumulate=True)
 
 
