@@ -1,31 +1,21 @@
-// Tree attention, float32 (tree_attention.cu says what is computed and how): fused multiply-adds on the CUDA cores.
+// Tree attention, float32 (tree_attention.cu says what is computed and how): products in two terms on the tensor cores.
 #include "tree_attention_tiles.cuh"
 
 namespace {
 
 template <int DP>
 int by_rows(const Args* a, long long pages, int tile_rows, int wide, int* info, cudaStream_t stream) {
-    if constexpr (DP <= 64) {
-        if (tile_rows == 4 && wide == 1) TREE_GO(float, 4, 1, 8, 32, 1, 1);
-        if (tile_rows == 4 && wide == 2) TREE_GO(float, 4, 1, 2, 32, 1, 6);
-        if (tile_rows == 4 && !wide) TREE_GO(float, 4, 1, 4, 32, 1, 3);
-        if (tile_rows == 8 && wide == 1) TREE_GO(float, 8, 1, 8, 32, 1, 1);
-        if (tile_rows == 8 && wide == 2) TREE_GO(float, 8, 1, 2, 32, 1, 5);
-        if (tile_rows == 8 && !wide) TREE_GO(float, 8, 1, 4, 32, 1, 3);
-        if (tile_rows == 16 && wide == 1) TREE_GO(float, 16, 1, 6, 32, 1, 1);
-        if (tile_rows == 16 && wide == 2) TREE_GO(float, 16, 1, 2, 32, 1, 4);
-        if (tile_rows == 16 && !wide) TREE_GO(float, 16, 1, 4, 32, 1, 2);
-    } else if constexpr (DP == 128) {
-        if (tile_rows == 4 && wide == 1) TREE_GO(float, 4, 1, 6, 32, 1, 1);
-        if (tile_rows == 4 && !wide) TREE_GO(float, 4, 1, 3, 32, 1, 2);
-        if (tile_rows == 8 && wide == 1) TREE_GO(float, 8, 1, 6, 32, 1, 1);
-        if (tile_rows == 8 && !wide) TREE_GO(float, 8, 1, 3, 32, 1, 2);
-        if (tile_rows == 16 && wide == 1) TREE_GO(float, 16, 1, 4, 32, 1, 1);
-        if (tile_rows == 16 && !wide) TREE_GO(float, 16, 1, 2, 32, 1, 2);
-    } else {
-        if (tile_rows == 4 && !wide) TREE_GO(float, 4, 1, 3, 32, 1, 1);
-        if (tile_rows == 8 && !wide) TREE_GO(float, 8, 1, 3, 32, 1, 1);
-        if (tile_rows == 16 && !wide) TREE_GO(float, 16, 1, 2, 32, 1, 1);
+    if (tile_rows == 16) {
+        if constexpr (DP <= 64) {
+            if (wide == 1) TREE_GO(float, 16, 1, 8, 32, 1, 1);
+            if (wide == 2) TREE_GO(float, 16, 1, 2, 32, 1, 5);
+            if (!wide) TREE_GO(float, 16, 1, 4, 32, 1, 3);
+        } else if constexpr (DP == 128) {
+            if (wide == 1) TREE_GO(float, 16, 1, 6, 32, 1, 1);
+            if (!wide) TREE_GO(float, 16, 1, 3, 32, 1, 2);
+        } else {
+            if (!wide) TREE_GO(float, 16, 1, 3, 32, 1, 1);
+        }
     }
     return mllm_fail(1, "tree_attention: no kernel takes tiles of %d rows (variant %d)", tile_rows, wide);
 }

@@ -22,13 +22,13 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool vali
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], const void* p) {
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t address) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s_u32(p)) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
 }
-__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], const void* p) {
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t address) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(s_u32(p)) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -38,10 +38,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
-}
-// Two fused multiply-adds of neighbouring 32-bit floats in one instruction.
-__device__ __forceinline__ void fma2(unsigned long long& c, unsigned long long a, unsigned long long b) {
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
 }
 __device__ __forceinline__ unsigned long long pair_of(float x, float y) {
     unsigned long long r;
@@ -77,7 +73,17 @@ template <int WR> __device__ __forceinline__ bool group_any(int group, bool x) {
     return r != 0;
 }
 
-constexpr int P_ROW = 36;                                   // float32: a row of weights, padded so that 4 rows start on other banks
+// A 32-bit float as two terms that the tensor cores take (11 bits each; they do not look at the lower 13 of a word): the float as it
+// is, of which they take its upper part, and what that leaves out, exactly; of the latter they drop at most 2 bits, 2^-22 of the value.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    hi = __float_as_uint(x);
+    lo = __float_as_uint(x - __uint_as_float(hi & 0xffffe000u));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
 template <typename T, int DP, int RW, int WR, int WK, int BK, int ST>
 struct Shape {
@@ -89,12 +95,12 @@ struct Shape {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr size_t q_bytes = (size_t)ROWS * ROW * sizeof(T);
     static constexpr size_t kv_bytes = (size_t)WK * ST * 2 * TILE * sizeof(T);
-    static constexpr size_t p_bytes = F32 ? (size_t)WK * WR * RW * P_ROW * 4 : 0;
-    static constexpr int MN = F32 ? RW / 4 : 2;             // rows whose maximum and sum a thread keeps
-    static constexpr int ON = F32 ? RW / 4 * (DP / 8) : DP / 2;
+    static_assert(RW == 16, "rows of an MMA");
+    static constexpr int MN = 2;                            // rows whose maximum and sum a thread keeps
+    static constexpr int ON = DP / 2;                       // and its elements of the result
     static constexpr int X_ROW = DP + 8;                    // the groups' results meet as rows of 32-bit floats
     static constexpr size_t xch_bytes = WK > 1 ? (size_t)WK * ROWS * (X_ROW + 2) * 4 : 0;
-    static constexpr size_t bytes = (kv_bytes + p_bytes > xch_bytes ? kv_bytes + p_bytes : xch_bytes) + q_bytes;
+    static constexpr size_t bytes = (kv_bytes > xch_bytes ? kv_bytes : xch_bytes) + q_bytes;
 };
 
 template <typename T, int DP, int RW, int WR, int WK, int BK, int ST, int PER_SM, bool TMA>
@@ -111,7 +117,6 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
     const int group = threadIdx.x / NT, gtid = threadIdx.x % NT, warp = gtid >> 5, lane = gtid & 31;
     T* sK = reinterpret_cast<T*>(smem) + (size_t)group * ST * 2 * TILE;
     T* sV = sK + ST * TILE;
-    float* sP = reinterpret_cast<float*>(smem + S::kv_bytes) + (size_t)(group * WR + warp) * RW * P_ROW;
     T* sQ = reinterpret_cast<T*>(smem + S::bytes - S::q_bytes);
     // element `d` of a buffer's row: 16-byte pieces of a block of 128 bytes stand in an order of the row's own
     auto at = [&](const T* buffer, int row, int d) {
@@ -242,29 +247,37 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
         __syncthreads();
 
         // ---- running state
-        float o[F32 ? 1 : ON];                                // bfloat16: the accumulators' fragments
-        unsigned long long o2[F32 ? ON / 2 : 1];              // float32: [MN][DP / 32][2] pairs of columns
+        float o[ON];                                          // the accumulators' fragments
 #pragma unroll
-        for (int i = 0; i < (F32 ? 1 : ON); ++i) o[i] = 0.f;
-#pragma unroll
-        for (int i = 0; i < (F32 ? ON / 2 : 1); ++i) o2[i] = 0ull;
+        for (int i = 0; i < ON; ++i) o[i] = 0.f;
         float m_run[MN], l_run[MN];
 #pragma unroll
         for (int i = 0; i < MN; ++i) { m_run[i] = -INFINITY; l_run[i] = 0.f; }
-        const int g = lane >> 2, tq = lane & 3;               // bfloat16: fragment row and column
-        const int rg = lane >> 3, kg = lane & 7;              // float32: row and key (or column) of a lane
-        uint32_t qa[F32 ? 1 : DP / 16][4];
+        const int g = lane >> 2, tq = lane & 3;               // fragment row and column
+        uint32_t qa[F32 ? 1 : DP / 16][4];                    // bfloat16: the queries' fragments
+        // float32: the terms of the 16 x 8 queries from column 8 ks on
+        auto split_queries = [&](int ks, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+            const T* q0 = sQ + (warp * 16 + g) * ROW + ks * 8 + tq;
+            split_tf32(to_f32(q0[0]), hi[0], lo[0]);
+            split_tf32(to_f32(q0[8 * ROW]), hi[1], lo[1]);
+            split_tf32(to_f32(q0[4]), hi[2], lo[2]);
+            split_tf32(to_f32(q0[8 * ROW + 4]), hi[3], lo[3]);
+        };
         if constexpr (!F32) {
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) ldsm_x4(qa[ks], sQ + (warp * 16 + (lane & 15)) * ROW + ks * 16 + (lane >> 4) * 8);
+            for (int ks = 0; ks < DP / 16; ++ks) ldsm_x4(qa[ks], s_u32(sQ + (warp * 16 + (lane & 15)) * ROW + ks * 16 + (lane >> 4) * 8));
         }
-        auto row_of = [&](int i) { return r0 + warp * RW + (F32 ? rg + 4 * i : g + 8 * i); };      // the query row of a thread's i-th state
+        auto row_of = [&](int i) { return r0 + warp * RW + g + 8 * i; };      // the query row of a thread's i-th state
         auto words_of = [&](int r) { return a.ancestors + (size_t)(first + (r < rows ? r / G : 0)) * a.words; };
 
         for (int use = TMA ? uses : 0; t <= t_last; t += WK, ++use) {
             const int stage = use % ST;
             T* tK = sK + stage * TILE;
             T* tV = sV + stage * TILE;
+            // Where a lane reads: its row and piece 0 of the first block of 128 bytes.  Another piece is that address with the piece's
+            // number xored into bits 4 to 6 (buffers start at multiples of 1,024 bytes), other rows and blocks are a constant away.
+            const uint32_t oK = (uint32_t)(reinterpret_cast<uint8_t*>(tK) - smem), oV = (uint32_t)(reinterpret_cast<uint8_t*>(tV) - smem);
+            auto piece_of = [](uint32_t lane_at, int piece) { return (lane_at ^ (uint32_t)((piece & 7) << 4)) + (uint32_t)((piece >> 3) * BK * 128); };
             const int key0 = t * BK;
             const bool tail = key0 + BK > min(len, keys);     // the tile reaches into the tree or past the keys
             mask_t seen[MN];
@@ -275,46 +288,53 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
             }
             wait(&k_full[TMA ? group : 0][stage], use);       // the tile's keys
             if (!TMA || WR > 1) group_sync<WR>(group);
-            float sc[F32 ? 4 * MN : BK / 2];                  // scores, then weights
+            float sc[BK / 2];                                 // scores, then weights
             if (active) {
                 if constexpr (!F32) {
                     // ---- S = Q K^T: 16 rows x BK keys
 #pragma unroll
                     for (int i = 0; i < BK / 2; ++i) sc[i] = 0.f;
+                    const uint32_t lk = s_u32(smem) + oK + ((lane & 7) + ((lane >> 4) << 3)) * 128 + (((lane & 7) ^ (lane >> 3 & 1)) << 4);
 #pragma unroll
                     for (int ks = 0; ks < DP / 16; ++ks) {
 #pragma unroll
                         for (int np = 0; np < BK / 16; ++np) {
                             uint32_t b[4];
-                            ldsm_x4(b, at(tK, np * 16 + (lane & 7) + ((lane >> 4) << 3), ks * 16 + ((lane >> 3) & 1) * 8));
+                            ldsm_x4(b, piece_of(lk, 2 * ks) + np * 2048);
                             mma16816(*reinterpret_cast<float (*)[4]>(&sc[8 * np]), qa[ks], b[0], b[1]);
                             mma16816(*reinterpret_cast<float (*)[4]>(&sc[8 * np + 4]), qa[ks], b[2], b[3]);
                         }
                     }
                 } else {
-                    // ---- S: rows rg + 4 i, keys kg + 8 j; even and odd columns in the halves of a pair
-                    unsigned long long s2[MN][4];
+                    // ---- S: three of the four products of terms, the small ones in sums of their own; the large ones in two, since
+                    // the unit cuts its sums off where the CUDA cores round them
+                    float c0[BK / 8][4], c1[BK / 8][4], cs[BK / 8][4];
 #pragma unroll
-                    for (int i = 0; i < MN; ++i)
+                    for (int nt = 0; nt < BK / 8; ++nt)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) s2[i][j] = 0ull;
-                    const float* qr = reinterpret_cast<const float*>(sQ) + (warp * RW + rg) * ROW;
-#pragma unroll 4
-                    for (int d = 0; d < DP; d += 4) {
-                        ulonglong2 qv[MN];
+                        for (int e = 0; e < 4; ++e) c0[nt][e] = c1[nt][e] = cs[nt][e] = 0.f;
+                    const uint32_t lk = oK + g * 128 + (g << 4) + tq * 4;
+#pragma unroll(DP <= 64 ? DP / 16 : 4)
+                    for (int k2 = 0; k2 < DP / 16; ++k2)
 #pragma unroll
-                        for (int i = 0; i < MN; ++i) qv[i] = *reinterpret_cast<const ulonglong2*>(qr + 4 * i * ROW + d);
+                        for (int half = 0; half < 2; ++half) {
+                            const int ks = 2 * k2 + half;
+                            uint32_t ah[4], al[4];
+                            split_queries(ks, ah, al);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const ulonglong2 kv = *reinterpret_cast<const ulonglong2*>(at(tK, kg + 8 * j, d));
-#pragma unroll
-                            for (int i = 0; i < MN; ++i) { fma2(s2[i][j], qv[i].x, kv.x); fma2(s2[i][j], qv[i].y, kv.y); }
+                            for (int nt = 0; nt < BK / 8; ++nt) {
+                                uint32_t bh0, bl0, bh1, bl1;
+                                split_tf32(*reinterpret_cast<const float*>(smem + piece_of(lk, 2 * ks) + nt * 1024), bh0, bl0);
+                                split_tf32(*reinterpret_cast<const float*>(smem + piece_of(lk, 2 * ks + 1) + nt * 1024), bh1, bl1);
+                                mma_tf32(half ? c1[nt] : c0[nt], ah, bh0, bh1);
+                                mma_tf32(cs[nt], ah, bl0, bl1);
+                                mma_tf32(cs[nt], al, bh0, bh1);
+                            }
                         }
-                    }
 #pragma unroll
-                    for (int i = 0; i < MN; ++i)
+                    for (int nt = 0; nt < BK / 8; ++nt)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) { const float2 h = halves(s2[i][j]); sc[4 * i + j] = h.x + h.y; }
+                        for (int e = 0; e < 4; ++e) sc[4 * nt + e] = (c0[nt][e] + c1[nt][e]) + cs[nt][e];
                 }
             }
             group_sync<WR>(group);                            // the keys' buffer is free
@@ -328,36 +348,17 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
 #pragma unroll
                 for (int i = 0; i < MN; ++i) {
                     float mx = -INFINITY;
-                    if constexpr (F32) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if (tail && !(seen[i] >> (kg + 8 * j) & 1)) sc[4 * i + j] = -INFINITY;
-                            mx = fmaxf(mx, sc[4 * i + j]);
+                    for (int nt = 0; nt < BK / 8; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            if (tail && !(seen[i] >> (nt * 8 + 2 * tq + e) & 1)) sc[4 * nt + 2 * i + e] = -INFINITY;
+                            mx = fmaxf(mx, sc[4 * nt + 2 * i + e]);
                         }
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                    } else {
-#pragma unroll
-                        for (int nt = 0; nt < BK / 8; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                if (tail && !(seen[i] >> (nt * 8 + 2 * tq + e) & 1)) sc[4 * nt + 2 * i + e] = -INFINITY;
-                                mx = fmaxf(mx, sc[4 * nt + 2 * i + e]);
-                            }
-                    }
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                     const float m_new = fmaxf(m_run[i], mx), use = m_new == -INFINITY ? 0.f : m_new;
-                    if constexpr (F32) {
-                        alpha[i] = exp2f((m_run[i] - use) * a.scale_log2);
-                        float sum = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float p = exp2f((sc[4 * i + j] - use) * a.scale_log2);
-                            sP[(rg + 4 * i) * P_ROW + kg + 8 * j] = p;
-                            sum += p;
-                        }
-                        l_run[i] = l_run[i] * alpha[i] + sum;          // this lane's keys; the lanes meet at the end
-                    } else {
+                    {
                         alpha[i] = fast_exp2((m_run[i] - use) * a.scale_log2);
                         const unsigned long long neg = pair_of(-use, -use), scale2 = pair_of(a.scale_log2, a.scale_log2);
                         unsigned long long sum = 0ull;
@@ -376,18 +377,8 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
                     m_run[i] = m_new;
                 }
                 if (__any_sync(0xffffffffu, moved)) {
-                    if constexpr (F32) {
 #pragma unroll
-                        for (int i = 0; i < MN; ++i)
-#pragma unroll
-                            for (int c = 0; c < DP / 16; ++c) {
-                                const float2 h = halves(o2[i * (DP / 16) + c]);
-                                o2[i * (DP / 16) + c] = pair_of(h.x * alpha[i], h.y * alpha[i]);
-                            }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < ON; ++i) o[i] *= alpha[i >> 1 & 1];
-                    }
+                    for (int i = 0; i < ON; ++i) o[i] *= alpha[i >> 1 & 1];
                 }
             }
 
@@ -415,6 +406,7 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
             if (active) {
                 // ---- O += P V
                 if constexpr (!F32) {
+                    const uint32_t lv = s_u32(smem) + oV + ((lane & 7) + (lane >> 3 & 1) * 8) * 128 + (((lane & 7) ^ (lane >> 4)) << 4);
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; ++kk) {
                         uint32_t pa[4], pb[4];
@@ -427,7 +419,7 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
 #pragma unroll
                         for (int dp = 0; dp < DP / 16; ++dp) {
                             uint32_t b[4];
-                            ldsm_x4_trans(b, at(tV, kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, dp * 16 + (lane >> 4) * 8));
+                            ldsm_x4_trans(b, piece_of(lv, 2 * dp) + kk * 2048);
                             float (&c0)[4] = *reinterpret_cast<float (*)[4]>(&o[8 * dp]);
                             float (&c1)[4] = *reinterpret_cast<float (*)[4]>(&o[8 * dp + 4]);
                             mma16816(c0, pa, b[0], b[1]);
@@ -437,31 +429,32 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
                         }
                     }
                 } else {
-                    __syncwarp();
-                    const float* pr = sP + rg * P_ROW;
-#pragma unroll 2
-                    for (int k = 0; k < BK; k += 4) {
-                        float4 p[MN];
+                    // the weights' fragments as they came: column t of an MMA stands for key 2 t, column t + 4 for key 2 t + 1.  A tile's
+                    // products are summed by themselves and added in rounded sums.
+                    uint32_t ph[BK / 8][4], pl[BK / 8][4];
 #pragma unroll
-                        for (int i = 0; i < MN; ++i) p[i] = *reinterpret_cast<const float4*>(pr + 4 * i * P_ROW + k);
+                    for (int s8 = 0; s8 < BK / 8; ++s8) {
+                        split_tf32(sc[4 * s8], ph[s8][0], pl[s8][0]);
+                        split_tf32(sc[4 * s8 + 2], ph[s8][1], pl[s8][1]);
+                        split_tf32(sc[4 * s8 + 1], ph[s8][2], pl[s8][2]);
+                        split_tf32(sc[4 * s8 + 3], ph[s8][3], pl[s8][3]);
+                    }
+                    const uint32_t lv0 = oV + 2 * tq * 128 + (((g >> 2) ^ (2 * tq)) << 4) + (g & 3) * 4,
+                                   lv1 = oV + (2 * tq + 1) * 128 + (((g >> 2) ^ (2 * tq + 1)) << 4) + (g & 3) * 4;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            unsigned long long pp[MN];
+                    for (int n8 = 0; n8 < DP / 8; ++n8) {
+                        float c0[4] = {0.f, 0.f, 0.f, 0.f}, cs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                            for (int i = 0; i < MN; ++i) {
-                                const float x = e == 0 ? p[i].x : e == 1 ? p[i].y : e == 2 ? p[i].z : p[i].w;
-                                pp[i] = pair_of(x, x);
-                            }
-#pragma unroll
-                            for (int c = 0; c < DP / 32; ++c) {
-                                const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(at(tV, k + e, c * 32 + kg * 4));
-#pragma unroll
-                                for (int i = 0; i < MN; ++i) {
-                                    fma2(o2[i * (DP / 16) + 2 * c], pp[i], v.x);
-                                    fma2(o2[i * (DP / 16) + 2 * c + 1], pp[i], v.y);
-                                }
-                            }
+                        for (int s8 = 0; s8 < BK / 8; ++s8) {
+                            uint32_t bh0, bl0, bh1, bl1;
+                            split_tf32(*reinterpret_cast<const float*>(smem + piece_of(lv0, 2 * n8) + s8 * 1024), bh0, bl0);
+                            split_tf32(*reinterpret_cast<const float*>(smem + piece_of(lv1, 2 * n8) + s8 * 1024), bh1, bl1);
+                            mma_tf32(c0, ph[s8], bh0, bh1);
+                            mma_tf32(cs, ph[s8], bl0, bl1);
+                            mma_tf32(cs, pl[s8], bh0, bh1);
                         }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[4 * n8 + e] += c0[e] + cs[e];
                     }
                 }
                 if (tail && odd) {
@@ -473,19 +466,12 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
                         for (int i = 0; i < MN; ++i) {
                             if (!(seen[i] >> b & 1)) continue;
 #pragma unroll
-                            for (int e = 0; e < (F32 ? DP / 16 : DP / 8); ++e) {
-                                const int d = F32 ? (e >> 1) * 32 + kg * 4 + 2 * (e & 1) : e * 8 + 2 * tq;
+                            for (int e = 0; e < DP / 8; ++e) {
+                                const int d = e * 8 + 2 * tq;
                                 if (d >= a.dh) continue;
-                                float x = to_f32(vrow[d]), y = to_f32(vrow[d + 1]);
-                                x = fabsf(x) < INFINITY ? 0.f : x;
-                                y = fabsf(y) < INFINITY ? 0.f : y;
-                                if constexpr (F32) {
-                                    const float2 h = halves(o2[i * (DP / 16) + e]);
-                                    o2[i * (DP / 16) + e] = pair_of(h.x + x, h.y + y);
-                                } else {
-                                    o[e * 4 + 2 * i] += x;
-                                    o[e * 4 + 2 * i + 1] += y;
-                                }
+                                const float x = to_f32(vrow[d]), y = to_f32(vrow[d + 1]);
+                                if (!(fabsf(x) < INFINITY)) o[e * 4 + 2 * i] += x;
+                                if (!(fabsf(y) < INFINITY)) o[e * 4 + 2 * i + 1] += y;
                             }
                         }
                     }
@@ -501,24 +487,9 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
         // the lanes' shares of the sums
 #pragma unroll
         for (int i = 0; i < MN; ++i) {
-            if (F32) l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 4);
             l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
             l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
         }
-        float res[ON];                                        // [MN][columns], a pair of neighbours after the other
-#pragma unroll
-        for (int i = 0; i < MN; ++i)
-#pragma unroll
-            for (int e = 0; e < ON / MN / 2; ++e) {
-                if constexpr (F32) {
-                    const float2 h = halves(o2[i * (DP / 16) + e]);
-                    res[i * (ON / MN) + 2 * e] = h.x;
-                    res[i * (ON / MN) + 2 * e + 1] = h.y;
-                } else {
-                    res[i * (ON / MN) + 2 * e] = o[e * 4 + 2 * i];
-                    res[i * (ON / MN) + 2 * e + 1] = o[e * 4 + 2 * i + 1];
-                }
-            }
         // ---- out: a thread's own elements where the block is one group; else the groups' rows meet in shared memory, in order, and
         // every thread finishes neighbours of a row
         auto put = [&](int r, int d, float x, float y, float m, float l, bool first_of_row) {
@@ -543,11 +514,11 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
 #pragma unroll
                 for (int i = 0; i < MN; ++i) {
                     const int r = group * S::ROWS + row_of(i) - r0;
-                    if ((F32 ? kg : tq) == 0) *reinterpret_cast<float2*>(xml + 2 * r) = make_float2(m_run[i], l_run[i]);
+                    if (tq == 0) *reinterpret_cast<float2*>(xml + 2 * r) = make_float2(m_run[i], l_run[i]);
 #pragma unroll
-                    for (int e = 0; e < ON / MN / 2; ++e) {
-                        const int d = F32 ? (e >> 1) * 32 + kg * 4 + 2 * (e & 1) : e * 8 + 2 * tq;
-                        *reinterpret_cast<float2*>(xch + r * X + d) = make_float2(res[i * (ON / MN) + 2 * e], res[i * (ON / MN) + 2 * e + 1]);
+                    for (int e = 0; e < DP / 8; ++e) {
+                        const int d = e * 8 + 2 * tq;
+                        *reinterpret_cast<float2*>(xch + r * X + d) = make_float2(o[e * 4 + 2 * i], o[e * 4 + 2 * i + 1]);
                     }
                 }
             }
@@ -580,9 +551,9 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
                 const int r = row_of(i);
                 if (r >= rows) continue;
 #pragma unroll
-                for (int e = 0; e < ON / MN / 2; ++e) {
-                    const int d = F32 ? (e >> 1) * 32 + kg * 4 + 2 * (e & 1) : e * 8 + 2 * tq;
-                    if (d < a.dh) put(r, d, res[i * (ON / MN) + 2 * e], res[i * (ON / MN) + 2 * e + 1], m_run[i], l_run[i], d == 0);
+                for (int e = 0; e < DP / 8; ++e) {
+                    const int d = e * 8 + 2 * tq;
+                    if (d < a.dh) put(r, d, o[e * 4 + 2 * i], o[e * 4 + 2 * i + 1], m_run[i], l_run[i], d == 0);
                 }
             }
         }

@@ -2421,7 +2421,7 @@ def draft_tables(lengths, cu_nodes, parents, pages, cu_pages, page_size: int, *,
 
 
 TREE_UNIT = 64               # keys of a unit of work of a tree attention that is cut along its keys
-TREE_JOIN_ROUNDS = {True: 2, False: 4}      # what the parts' join and the changes between them cost, in rounds of a block (float32, bfloat16)
+TREE_JOIN_ROUNDS = {True: 3, False: 4}      # what the parts' join and the changes between them cost, in rounds of a block (float32, bfloat16)
 
 
 @functools.lru_cache(maxsize=256)
@@ -2450,7 +2450,7 @@ def tree_plan(float32: bool, S: int, num_heads: int, num_kv_heads: int, head_dim
     1,008: 15.3 in blocks of their own, 18.7 shared; 64 pairs of up to 8,004 (heads of 128): 103 and 41."""
     rows = max(1, max_nodes * (num_heads // num_kv_heads))
     if float32:
-        tile = next((t for t in (4, 8) if rows <= t), 16)
+        tile = 16
     elif boxes and head_dim <= 128:
         tile = 16 if rows <= (32 if head_dim <= 64 else 16) else 128 if rows <= 128 else 256
     else:
