@@ -94,6 +94,65 @@ int launch_join(const Args& a, cudaStream_t stream) {
     return 0;
 }
 
+// The same for the tiles of the tcgen05 kernel, whose threads hold a row each: sums lie four columns of all rows at a time
+// ([slot][columns / 4][row][4]), so that a warp's 32 rows are 512 neighbouring bytes where it writes them (as rows, 32 pieces of 16
+// bytes in lines of their own: 256 rows of 128, 8 us a block).  A thread takes four columns of a row, R rows a block.
+template <int R>
+__global__ void __launch_bounds__(256)
+tree_attention_join_tall_kernel(const Args a) {
+    pdl_wait();
+    pdl_launch();
+    const int quad = threadIdx.x / R, quads = a.dh / 4, G = a.G;
+    const int4* record = reinterpret_cast<const int4*>(a.cuts + blockIdx.x + 1);
+    const int4 r0 = record[0], r1 = record[1];
+    const Cut cut{r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+    const int here_rows = min(a.tile_rows, cut.rows - cut.row0);
+    if (cut.parts == 0 || quad >= quads) return;
+    for (int row = blockIdx.y * R + threadIdx.x % R; row < here_rows; row += gridDim.y * R) {
+        constexpr int AHEAD = 8;
+        float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int p0 = 0; p0 < cut.parts; p0 += AHEAD) {
+            float2 ml[AHEAD];
+            float4 v[AHEAD];
+#pragma unroll
+            for (int e = 0; e < AHEAD; ++e) {
+                const int p = min(p0 + e, cut.parts - 1);
+                const size_t slot = cut.slot + 2 * p + (p == 0 ? cut.shift : 0);
+                ml[e] = *reinterpret_cast<const float2*>(a.part_ml + 2 * (slot * a.tile_rows + row));
+                v[e] = *reinterpret_cast<const float4*>(a.part_o + 4 * ((slot * quads + quad) * a.tile_rows + row));
+            }
+            float m_new = m;
+#pragma unroll
+            for (int e = 0; e < AHEAD; ++e) m_new = fmaxf(m_new, ml[e].x);
+            const float use = m_new == -INFINITY ? 0.f : m_new, keep = exp2f((m - use) * a.scale_log2);
+            m = m_new;
+            l *= keep;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[x] *= keep;
+#pragma unroll
+            for (int e = 0; e < AHEAD; ++e) {
+                const float w = p0 + e < cut.parts ? exp2f((ml[e].x - use) * a.scale_log2) : 0.f;
+                if (w == 0.f) continue;
+                l = fmaf(ml[e].y, w, l);
+                o[0] = fmaf(v[e].x, w, o[0]);
+                o[1] = fmaf(v[e].y, w, o[1]);
+                o[2] = fmaf(v[e].z, w, o[2]);
+                o[3] = fmaf(v[e].w, w, o[3]);
+            }
+        }
+        const float inv = inverse_sum(l);
+        const int q = cut.row0 + row;
+        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + (size_t)(cut.first + q / G) * a.ldo + (size_t)(cut.hk * G + q % G) * a.dh + 4 * quad;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) to[x] = __float2bfloat16(o[x] * inv);
+    }
+}
+int launch_join_tall(const Args& a, cudaStream_t stream) {
+    if (a.blocks < 2) return 0;
+    if (a.dh <= 64) MLLM_CUDA(mllm_launch(tree_attention_join_tall_kernel<16>, dim3(a.blocks - 1, (a.max_rows + 15) / 16), dim3(256), 0, stream, true, a));
+    else MLLM_CUDA(mllm_launch(tree_attention_join_tall_kernel<8>, dim3(a.blocks - 1, (a.max_rows + 7) / 8), dim3(256), 0, stream, true, a));
+    return 0;
+}
 
 // Variants by how many blocks there are: `wide` 1 has the most groups (a block per pair, fewer pairs than SMs), 2 the fewest.
 template <int DP>
@@ -126,6 +185,7 @@ int by_head(const Args* a, int dh, long long pages, int tile_rows, int wide, int
 }  // namespace
 
 int tree::join(const Args& a, int dtype, cudaStream_t stream) {
+    if (a.tile_rows >= 128) return launch_join_tall(a, stream);
     return dtype == MLLM_F32 ? launch_join<float>(a, stream) : launch_join<__nv_bfloat16>(a, stream);
 }
 
@@ -168,7 +228,7 @@ struct TreeAttentionArgs {
     void* out;
     float *part_o, *part_ml;
     Cut* cuts;
-    long long ldq, ldo, pages, bt_stride, width, words, S, H, Hkv, dh, page_size, tile_rows, max_rows, unit, least, blocks, wide, dtype;
+    long long ldq, ldo, pages, bt_stride, width, words, S, H, Hkv, dh, page_size, tile_rows, max_rows, unit, least, blocks, gap, wide, dtype;
     double scale;
 };
 MLLM_EXPORT int mllm_tree_attention(const TreeAttentionArgs* p, cudaStream_t stream) {
@@ -179,7 +239,7 @@ MLLM_EXPORT int mllm_tree_attention(const TreeAttentionArgs* p, cudaStream_t str
     if (dh < 16 || dh > 256 || dh % 16) return mllm_fail(1, "tree_attention: head size %d is not a multiple of 16 in 16..256", dh);
     if (!(scale > 0.f)) return mllm_fail(1, "tree_attention: the score scale must be positive, got %g", (double)scale);
     if (dtype != MLLM_F32 && dtype != MLLM_BF16) return mllm_fail(1, "tree_attention: unknown dtype code %d", dtype);
-    if (p->page_size <= 0 || p->width <= 0 || p->words <= 0 || p->unit < 64 || p->least <= 0 || (p->unit & (p->unit - 1)) || p->blocks < 0 || p->max_rows <= 0 ||
+    if (p->page_size <= 0 || p->width <= 0 || p->words <= 0 || p->unit < 64 || p->least <= 0 || (p->unit & (p->unit - 1)) || p->blocks < 0 || p->gap < 0 || p->max_rows <= 0 ||
         p->tile_rows <= 0 || (p->tile_rows & (p->tile_rows - 1)))
         return mllm_fail(1, "tree_attention: pages of %lld, a table of %lld columns, %lld words, units of %lld keys, %lld blocks, %lld rows",
                          p->page_size, p->width, p->words, p->unit, p->blocks, p->max_rows);
@@ -198,7 +258,7 @@ MLLM_EXPORT int mllm_tree_attention(const TreeAttentionArgs* p, cudaStream_t str
     const Args a{p->q, p->ldq, p->k_pages, p->v_pages, p->block_table, (int)p->bt_stride, (int)p->width, p->lengths, p->cu_nodes, p->ancestors,
                  (int)p->words, p->out, p->ldo, p->part_o, p->part_ml, p->cuts, (int)p->S, H, Hkv, H / Hkv, dh, page_size,
                  shifts ? 31 - __builtin_clz(page_size) : -1, (uintptr_t)p->q % 16 == 0 && p->ldq * es % 16 == 0, out_vec, tile_rows,
-                 31 - __builtin_clz(tile_rows), (int)(p->max_rows < tile_rows ? p->max_rows : tile_rows), 31 - __builtin_clz((int)p->unit), (int)p->least, (int)p->blocks,
+                 31 - __builtin_clz(tile_rows), (int)(p->max_rows < tile_rows ? p->max_rows : tile_rows), 31 - __builtin_clz((int)p->unit), (int)p->least, (int)p->blocks, (int)p->gap,
                  (int)max_tiles, scale * LOG2E};
     if (dtype == MLLM_F32) return tree::f32(&a, dh, p->pages, tile_rows, (int)p->wide, nullptr, stream);
     if (tile_rows >= 128) return tcgen05(a, p->pages, stream);

@@ -14,12 +14,12 @@ struct Args {
     const int* block_table; int bt_stride, width;
     const int* lengths; const int* cu_nodes; const int* ancestors; int words;
     void* out; long long ldo;
-    float* part_o; float* part_ml;          // [2 * blocks, tile rows, dh] and [2 * blocks, tile rows, 2]
+    float* part_o; float* part_ml;          // [2 * blocks, tile rows, dh] (tree_attention.cu says in what order) and [2 * blocks, tile rows, 2]
     struct Cut* cuts;                       // [blocks]
     int S, H, Hkv, G, dh, page_size, page_shift;
     int q_vec, out_vec;                     // queries can be read 16 bytes at a time; elements that a store may write at once
     int tile_rows, tile_shift, max_rows;    // query rows of a tile (a power of two), and those of the largest tree's first
-    int unit_shift, least, blocks;          // keys per unit of work, the least of them for a block, blocks (0: one per pair)
+    int unit_shift, least, blocks, gap;     // keys per unit of work, the least of them for a block, blocks (0: one per pair), a pair's own cost in units
     int max_tiles;
     float scale_log2;
 };
@@ -31,11 +31,12 @@ struct Cut { int parts, first, hk, row0, rows, slot, shift, unused; };      // s
 // ------------------------------------------------------------------------------------------------ how the work is cut
 // A pair is a tile of query rows of one (request, key/value head).  Either every pair has a block of its own (blocks == 0: the grid
 // is (head and tile, request)), or the pairs' keys are shared out evenly: each pair's keys in units of 2^unit_shift, all units of all pairs
-// in one line, in order of request, head, tile and position, and every block takes as many neighbours of that line as any other
-// (or one less), whatever the lengths, but no fewer than its groups or streams can walk at once.  A block's share of one pair is a segment.  Pairs that lie in one block are finished there;
-// the others leave their segments' sums in scratch, two slots a block (only its first and last segment can be parts of a pair), and
-// the join kernel adds them in order of position.  A
-// block finds its place by a scan over the requests, 32 at a time.
+// in one line, in order of request, head, tile and position, before each pair's a gap for what the pair costs beside its keys (without
+// gaps, blocks that got many short texts held up the rest: 24 requests of 200 to 3,000 keys, 12 heads, 40 rows: 95 us, with them 56).
+// Every block takes as long a piece of that line as any other (or one unit less), whatever the lengths, but no fewer units than its
+// groups or streams can walk at once.  A block's share of one pair is a segment.  Pairs that lie in one block are finished there; the
+// others leave their segments' sums in scratch, two slots a block (only its first and last segment can be parts of a pair), and the
+// join kernel adds them in order of position.  A block finds its place by a scan over the requests, 32 at a time.
 struct Request { int s, first, n, len, keys, units, tiles; };
 
 __device__ __forceinline__ int keys_of(const Args& a, int len, int n) {     // those that the block table holds
@@ -54,7 +55,9 @@ __device__ __forceinline__ Request request_of(const Args& a, int s) {
     }
     return r;
 }
-__device__ __forceinline__ unsigned int weight_of(const Args& a, const Request& r) { return (unsigned int)r.units * r.tiles * a.Hkv; }
+__device__ __forceinline__ unsigned int weight_of(const Args& a, const Request& r) {
+    return (unsigned int)(r.units + a.gap) * r.tiles * a.Hkv;
+}
 
 struct Line {                               // the line of units, shared out among blocks: the first `extra` of them take per + 1
     unsigned int units, blocks, per, extra;
@@ -137,25 +140,28 @@ __device__ __forceinline__ void fill(const Args& a, Segments* l) {              
         unsigned int base = 0;
         Request r{};
         bool have = false;
-        for (; at < end && count < Segments::CAP; ++count) {
+        while (at < end && count < Segments::CAP) {
             if (!have || at - base >= weight_of(a, r)) r = find(a, line, at, &base);
             have = true;
-            const unsigned int pair = (at - base) / r.units, unit = at - base - pair * r.units, take = min(r.units - unit, end - at);
-            const unsigned int hk = pair / r.tiles;
+            const unsigned int each = r.units + a.gap, pair = (at - base) / each, hk = pair / r.tiles;
+            const unsigned int from = base + pair * each + a.gap, to = from + r.units;        // the pair's units, behind its gap
+            const unsigned int u0 = max(at, from), u1 = min(to, end);
             if (opening && at == begin && lane == 0) {
-                const unsigned int from = at - unit, c0 = blockIdx.x - 1;
+                const unsigned int c0 = blockIdx.x - 1;
                 Cut cut{0, r.first, (int)hk, (int)(pair - hk * r.tiles) * a.tile_rows, r.n * a.G, 2 * (int)c0, 0, 0};
-                if (unit && line.begin(c0) <= from) {
-                    cut.parts = (int)(line.block_of(from + r.units - 1) - c0) + 1;
-                    cut.shift = line.begin(c0) < from ? 1 : 0;        // block c0's segment is its last one, unless it begins with it
+                if (u0 > from && line.begin(c0) <= from) {
+                    cut.parts = (int)(line.block_of(to - 1) - c0) + 1;
+                    cut.shift = line.begin(c0) + a.gap < from ? 1 : 0;      // block c0's segment is its last one, unless it is its first
                 }
                 a.cuts[blockIdx.x] = cut;
             }
+            at = min(to, end);
+            if (u0 >= u1) continue;                               // the block ends in the gap
             if (lane == 0)
                 l->list[count] = Segment{r.s, r.first, r.n, r.len, r.keys, (int)hk, (int)(pair - hk * r.tiles) * a.tile_rows, r.n * a.G,
-                                         (int)(unit << a.unit_shift), (int)min((long long)(unit + take) << a.unit_shift, (long long)r.keys),
-                                         take == (unsigned int)r.units ? -1 : 2 * (int)blockIdx.x + (at == begin ? 0 : 1)};
-            at += take;
+                                         (int)((u0 - from) << a.unit_shift), (int)min((long long)(u1 - from) << a.unit_shift, (long long)r.keys),
+                                         u1 - u0 == (unsigned int)r.units ? -1 : 2 * (int)blockIdx.x + (opening && count == 0 ? 0 : 1)};
+            ++count;
         }
         more = at < end;
     }

@@ -457,8 +457,9 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                 }
                 const int q = sg.row0 + tile_row;
                 const float inv = tree::inverse_sum(l);
-                const size_t pr = (size_t)max(sg.slot, 0) * a.tile_rows + tile_row;
-                if (sg.slot >= 0 && tile_row < rows && ks == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = make_float2(m, l);
+                const size_t slot = max(sg.slot, 0);
+                if (sg.slot >= 0 && tile_row < rows && ks == 0)
+                    *reinterpret_cast<float2*>(a.part_ml + 2 * (slot * a.tile_rows + tile_row)) = make_float2(m, l);
                 bf* orow = static_cast<bf*>(a.out) + (size_t)(sg.first + node) * a.ldo + (size_t)(sg.hk * G + q % G) * a.dh;
 #pragma unroll 1
                 for (int c0 = ks * (DP / KS); c0 < (ks + 1) * (DP / KS) && c0 < a.dh; c0 += 16) {
@@ -494,7 +495,8 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                     if (sg.slot >= 0) {
 #pragma unroll
                         for (int e = 0; e < 16; e += 4)
-                            *reinterpret_cast<float4*>(a.part_o + pr * a.dh + c0 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                            *reinterpret_cast<float4*>(a.part_o + 4 * ((slot * (a.dh / 4) + (c0 + e) / 4) * a.tile_rows + tile_row)) =
+                                make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                     } else {
                         uint32_t h[8];
 #pragma unroll

@@ -2362,7 +2362,7 @@ def _attend(impl, q, ldq, k_pages, v_pages, block_table, bt_stride, ctx, out, ld
 # that a step can follow the one before it without the host knowing how many tokens that one kept.  A request may bring no row.
 # Arguments go to C as one block of 64-bit fields (csrc/draft.cu): converted one by one they would take longer than the launch.
 DRAFT_MAX_NODES = 256
-_PACK_TABLES, _PACK_TREE, _PACK_ACCEPT, _PACK_KEEP = (struct.Struct(f) for f in ("15q", "29qd", "18q", "15q"))
+_PACK_TABLES, _PACK_TREE, _PACK_ACCEPT, _PACK_KEEP = (struct.Struct(f) for f in ("15q", "30qd", "18q", "15q"))
 
 
 def _i32(name: str, t) -> int:
@@ -2421,7 +2421,14 @@ def draft_tables(lengths, cu_nodes, parents, pages, cu_pages, page_size: int, *,
 
 
 TREE_UNIT = 64               # keys of a unit of work of a tree attention that is cut along its keys
-TREE_JOIN_ROUNDS = {True: 3, False: 4}      # what the parts' join and the changes between them cost, in rounds of a block (float32, bfloat16)
+# What a pair of tile and key/value head costs beside its keys where the keys are shared out (its queries, its first and last products,
+# its sums), in units; float32, bfloat16.  24 requests of 200 to 3,000 keys, 40 rows, 12 heads of 64: 95 us without it, 56 with 8 units.
+TREE_GAP = {True: 3, False: 8}
+# What a round of a block costs (by variant, or by tile in tensor memory), what comes before the first, and what the parts' join and the
+# changes between them cost (float32, bfloat16; of 0.7 where blocks are wide): all as rounds of variant 0.
+TREE_ROUND = {0: 1.0, 1: 1.2, 2: 1.0, 128: 0.9, 256: 0.7}
+TREE_START = {128: 1.0, 256: 4.0}
+TREE_JOIN_ROUNDS = {True: 2.0, False: 4.0}
 
 
 @functools.lru_cache(maxsize=256)
@@ -2438,37 +2445,37 @@ def tree_plan(float32: bool, S: int, num_heads: int, num_kv_heads: int, head_dim
     """How a tree attention is cut: (query rows of a tile, those of the largest tree, blocks that share the keys evenly (0: one for
     every pair of tile and key/value head), units that a block takes at least, variant).  ``boxes``: pages come by TMA.
 
-    Tiles.  float32: the smallest of 4, 8 and 16 that holds a tree's rows of one key/value head (more rows are more tiles: keys and
-    values come from L2 again, which costs less than warps that wait for one another; 5 requests, up to 37 rows, 25 heads of 64:
-    166 us in tiles of 16, 257 in tiles of 64).  bfloat16: tiles of 16 on mma.sync while few are needed, tensor memory beyond
-    (32 rows, 8 requests, 12 heads of 64: 15.6 us in two tiles of 16, 16.9; 64 rows: 19.7 and 19.4; heads of 128, 32 over 8, 32 rows:
-    37.4 and 31.4), except for heads over 128 and pages that no box fits.
+    Tiles.  float32: 16 rows (more rows are more tiles: keys and values come from L2 again).  bfloat16: 16 on mma.sync while one
+    holds a tree's rows, 128 and 256 in tensor memory beyond, where it takes the heads and pages; for heads of up to 64 and up to 64
+    rows, and for over 128 rows, whichever the rounds say (40 rows, 12 heads of 64: 4 requests of 500 keys 10.4 us in tiles of 16,
+    13.5 in one of 128; 24 of up to 3,000: 62.9 and 55.6.  256 rows of 32 heads of 128 over 8: 1 request of 6,000 keys 33 us in a
+    tile of 256, 27 in two of 128; 64 of up to 2,000: 158 and 181).
 
     Blocks.  A round is what a block walks at once.  A block per pair takes as many as the longest request, times the waves of
     pairs; sharing the keys out evenly takes their sum, and the join.  Variants differ in groups per block: 1, more groups for few
-    pairs, 2, fewer for many blocks.  12 pairs of 518 keys: 9.3 us in wide blocks, 10.7 in others, 13.4 shared; 192 pairs of up to
-    1,008: 15.3 in blocks of their own, 18.7 shared; 64 pairs of up to 8,004 (heads of 128): 103 and 41."""
+    pairs, 2, fewer for many blocks.  12 pairs of 518 keys: 9.2 us in wide blocks, 10.7 in others, 10.7 shared; 192 pairs of up to
+    1,008: 14.6 in blocks of their own, 17.0 shared; 64 pairs of up to 8,004 (heads of 128): 112 and 40.  Over 104 shapes the variant
+    that this picks took 1.4 % more than the fastest, and 15 % at most."""
     rows = max(1, max_nodes * (num_heads // num_kv_heads))
-    if float32:
-        tile = 16
+    if float32 or rows <= 16:
+        tiles = (16,)
     elif boxes and head_dim <= 128:
-        tile = 16 if rows <= (32 if head_dim <= 64 else 16) else 128 if rows <= 128 else 256
+        tiles = (128, 256) if rows > 128 else (16, 128) if rows <= 64 and head_dim <= 64 else (128,)
     else:
-        tile = 16 if rows <= 16 else 32 if rows <= 64 or head_dim > 128 else 64
-    pairs, keys, best = S * num_kv_heads * -(-rows // tile), max_length + max_nodes, None
-    for wide in (0, 1, 2):
-        v = _tree_variant(float32, head_dim, tile, wide)
-        if v is None:
-            continue
-        places, at_once = v[0] * sms, v[1]
-        own = -(-pairs // places) * -(-keys // at_once)
-        shared = -(-pairs * keys // (places * at_once))
-        if best is None or own < best[0]:
-            best = own, (tile, rows, 0, 1, wide)
-        if wide == 0 or (wide == 2 and shared >= 8 and head_dim <= 64):
-            cost = shared + TREE_JOIN_ROUNDS[float32] - (0.5 if wide == 2 else 0)
-            if cost < best[0]:
-                best = cost, (tile, rows, places, max(1, at_once // TREE_UNIT), wide)
+        tiles = (32,) if rows <= 64 or head_dim > 128 else (64,)
+    keys, best = max_length + max_nodes, None
+    for tile in tiles:
+        pairs = S * num_kv_heads * -(-rows // tile)
+        for wide in (0, 1, 2):
+            v = _tree_variant(float32, head_dim, tile, wide)
+            if v is None:
+                continue
+            places, at_once = v[0] * sms, v[1]
+            each, start = TREE_ROUND[tile if tile in TREE_START else wide], TREE_START.get(tile, 0.0)
+            for blocks, cost in ((0, each * -(-pairs // places) * -(-keys // at_once)),
+                                 (places, each * pairs * keys / (places * at_once) + TREE_JOIN_ROUNDS[float32] * (0.7 if wide == 1 else 1.0))):
+                if best is None or cost + start < best[0]:
+                    best = cost + start, (tile, rows, blocks, max(1, at_once // TREE_UNIT) if blocks else 1, wide)
     return best[1]
 
 
@@ -2520,7 +2527,7 @@ def tree_attention(q, k_pages, v_pages, block_table, lengths, cu_nodes, ancestor
     attention_launches["tree"] = attention_launches.get("tree", 0) + 1
     _call("mllm_tree_attention", _PACK_TREE.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), p_len, p_cu, p_anc, out.data_ptr(), part_o, part_ml, cuts,
-        ldq, ldo, P, bt_stride, width, words, S, num_heads, num_kv_heads, head_dim, ps, tile, rows, TREE_UNIT, least, blocks, wide, dt, scale),
+        ldq, ldo, P, bt_stride, width, words, S, num_heads, num_kv_heads, head_dim, ps, tile, rows, TREE_UNIT, least, blocks, TREE_GAP[dt == F32] if blocks else 0, wide, dt, scale),
         _stream())
     if blocks:
         launches += 1           # the kernel in which the parts meet
