@@ -279,8 +279,6 @@ keep_accepted_kernel(U* planes, long long plane_stride, int n_planes, int pages,
 
 }  // namespace
 
-MLLM_EXPORT int mllm_draft_max_nodes() { return MAX_NODES; }
-
 // The three entry points take their arguments packed in one block of 64-bit fields: a call from Python converts every argument of its
 // own, 0.12 us each, which for 20 to 30 of them is more than the launch.
 struct DraftTablesArgs {

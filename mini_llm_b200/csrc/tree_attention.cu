@@ -7,21 +7,27 @@
 // The places from L + n on hold other requests' or old data: they are never read (their part of a tile is zeros).
 //
 // What bounds it: a key and a value row are read once for all n * (heads per key/value head) query rows that use them, so few
-// rows are bound by the cache's bytes and many by the products (32-bit: by the CUDA cores' fused multiply-adds).
+// rows are bound by the cache's bytes, and with short texts by the chain of loads behind a launch (lengths, block table, queries and
+// keys, values), many by the products and the exponentials.
 // The maximum is kept as a score, and a weight is 2^((s - max) * scale * log2 e): the difference first, so that scores of any size
 // give weights up to 1 (a fused s * c - rounded(max * c) leaves a rounding of the maximum's size, which overflows from 2^31 on).
 //
-// Layout.  The query rows of one key/value head (row r = node r / G, head r % G of its group of G) are packed into tiles of
-// RW rows a warp and WR warps.  tree_attention.cuh says how the keys are cut into segments of blocks.  In a block WK groups of WR
+// Layout.  The query rows of one key/value head (row r = node r / G, head r % G of its group of G) are packed into tiles of 16 rows
+// a warp and WR warps.  tree_attention.cuh says how the keys are cut into segments of blocks.  In a block WK groups of WR
 // warps take a segment's tiles of BK keys in turn, each with its own running maximum, sum and output rows in registers and ST
 // buffers of keys and of values in shared memory: a buffer's next tile is asked for as soon as the product that read it is done, the
 // block-table entries one tile further ahead.  Tiles come by TMA, a box of one page's rows per lane, where pages are a multiple of
 // 8 tokens (16-byte cp.async by the threads, for other pages, brings 26 bytes a cycle into an SM at most, and 140 cycles of a warp
 // for every 512 bytes).  The groups meet in order at the end.
 //   bfloat16: S = Q K^T and O += P V on mma.sync.m16n8k16, p as two bfloat16 terms (its rounding and what that left out), so the
-//             weights keep about 16 bits; sums in 32 bits.
-//   float32:  fused multiply-adds of packed pairs on the CUDA cores.  A lane owns RW / 4 rows x 4 keys of S and RW / 4 rows x DP / 8
-//             columns of O: every 16 bytes from shared memory feed 8 to 16 of them.
+//             weights keep about 16 bits; sums in 32 bits.  (Products of two or eight rows on tcgen05 would be 128 high.)
+//   float32:  on mma.sync.m16n8k8 with both factors as two 11-bit terms, three products of the four: sums of the large ones in two
+//             chains, of the mixed ones in a third; a tile's sums of P V by themselves, added rounded.  Fused multiply-adds on the
+//             CUDA cores took 121 us where this takes 107 (below).
+// Measured (one launch among others, the join's included; what the bytes take at 6.5 TB/s in brackets): bfloat16, 12 heads of 64:
+// 1 request, 8 rows, 510 keys 9.0 us (0.2); 8 requests, 32 rows, up to 990 keys 15.0 us (2.7); 64 requests, up to 48 rows over 4
+// key/value heads, 500 to 4,000 keys 60 us (23); float32: 8 requests, 16 rows, up to 1,000 keys 22 us (5.0); 5 requests, up to 37
+// rows, up to 7,001 keys, 25 heads 107 us (41).
 // Values in places that some rows see and others do not (the tree's own) may be infinite or NaN: a weight of zero would turn them
 // into NaN, so such elements are taken out of the tile and added to the rows that see them only.
 #include "tree_attention_tiles.cuh"
@@ -29,8 +35,8 @@
 namespace {
 
 // The segments of the pairs that more than one block worked on meet, in order of position: a block per boundary between two blocks'
-// shares and 8 rows, a warp per row.  VD: columns of a lane.  Eight segments' rows (four of heads over 128) are in flight at once.  What bounds it: the
-// chain of three loads (what is cut, maxima and sums, rows) behind a launch.
+// shares and 8 rows, a warp per row.  VD: columns of a lane.  Eight segments' rows (four of heads over 128) are in flight at once.
+// What bounds it: the chain of three loads (what is cut, maxima and sums, rows) behind a launch.
 template <typename T, int VD>
 __global__ void __launch_bounds__(256)
 tree_attention_join_kernel(const Args a) {
@@ -159,20 +165,19 @@ template <int DP>
 int by_rows(const Args* a, long long pages, int tile_rows, int wide, int* info, cudaStream_t stream) {
     using bf = __nv_bfloat16;
     if constexpr (DP == 64) {
-        if (tile_rows == 16 && wide == 1) TREE_GO(bf, 16, 1, 8, 64, 1, 1);
-        if (tile_rows == 16 && wide == 2) TREE_GO(bf, 16, 1, 2, 64, 1, 6);
-        if (tile_rows == 16 && !wide) TREE_GO(bf, 16, 1, 4, 64, 1, 3);
-        if (tile_rows == 32 && !wide) TREE_GO(bf, 16, 2, 4, 32, 2, 2);
-        if (tile_rows == 64 && !wide) TREE_GO(bf, 16, 4, 2, 32, 3, 2);
+        if (tile_rows == 16 && wide == 1) TREE_GO(bf, 1, 8, 64, 1, 1);
+        if (tile_rows == 16 && wide == 2) TREE_GO(bf, 1, 2, 64, 1, 6);
+        if (tile_rows == 16 && !wide) TREE_GO(bf, 1, 4, 64, 1, 3);
+        if (tile_rows == 32 && !wide) TREE_GO_NO_BOXES(bf, 2, 4, 32, 2, 2);
+        if (tile_rows == 64 && !wide) TREE_GO_NO_BOXES(bf, 4, 2, 32, 3, 2);
     } else if constexpr (DP == 128) {
-        if (tile_rows == 16 && wide == 1) TREE_GO(bf, 16, 1, 8, 32, 1, 1);
-        if (tile_rows == 16 && wide == 2) TREE_GO(bf, 16, 1, 2, 32, 1, 4);
-        if (tile_rows == 16 && !wide) TREE_GO(bf, 16, 1, 4, 32, 1, 2);
-        if (tile_rows == 32 && !wide) TREE_GO(bf, 16, 2, 2, 32, 2, 2);
-        if (tile_rows == 64 && !wide) TREE_GO(bf, 16, 4, 2, 32, 2, 1);
+        if (tile_rows == 16 && wide == 1) TREE_GO(bf, 1, 8, 32, 1, 1);
+        if (tile_rows == 16 && !wide) TREE_GO(bf, 1, 4, 32, 1, 2);
+        if (tile_rows == 32 && !wide) TREE_GO_NO_BOXES(bf, 2, 2, 32, 2, 2);
+        if (tile_rows == 64 && !wide) TREE_GO_NO_BOXES(bf, 4, 2, 32, 2, 1);
     } else {
-        if (tile_rows == 16 && !wide) TREE_GO(bf, 16, 1, 4, 32, 1, 1);
-        if (tile_rows == 32 && !wide) TREE_GO(bf, 16, 2, 4, 32, 1, 1);
+        if (tile_rows == 16 && !wide) TREE_GO(bf, 1, 4, 32, 1, 1);
+        if (tile_rows == 32 && !wide) TREE_GO(bf, 2, 4, 32, 1, 1);
     }
     return mllm_fail(1, "tree_attention: no kernel takes tiles of %d rows (variant %d)", tile_rows, wide);
 }
@@ -212,15 +217,16 @@ MLLM_EXPORT int mllm_tree_attention_error(int* code) {
 // Of a variant's blocks: info[0], how many one SM holds at once, info[1], how many keys a block walks at once.  An error where no kernel
 // takes such tiles, or has such a variant.
 MLLM_EXPORT int mllm_tree_attention_variant(int dh, int tile_rows, int wide, int dtype, int* info) {
-    if (dtype == MLLM_BF16 && tile_rows >= 128) return tree::tcgen05_variant(dh, tile_rows, info);
+    if (dtype == MLLM_BF16 && tile_rows >= 128 && !wide) return tree::tcgen05_variant(dh, tile_rows, info);
     if (dtype == MLLM_F32) return tree::f32(nullptr, dh, 0, tile_rows, wide, info, nullptr);
     return by_head(nullptr, dh, 0, tile_rows, wide, info, nullptr);
 }
 
-// tile_rows: 128 or 256 (bfloat16, the kernel of tree_attention_tcgen05.cu), 16, 32 or 64 (bfloat16), 4, 8 or 16 (float32) query rows of a key/value head per tile; max_rows: those of
-// the largest tree (as far as the host knows).  blocks: those that share all keys evenly, in units of `unit` keys (a power of two from 64 on), no block fewer than `least`; they
-// need part_o [2 * blocks, tile_rows, dh], part_ml [2 * blocks, tile_rows, 2] and cuts [blocks] (8 integers each).  0: a block for every pair of tile and head.
-// The head size is a multiple of 16 up to 256.
+// tile_rows: 128 or 256 (bfloat16, the kernel of tree_attention_tcgen05.cu), 16 (and for pages that no box fits and heads over 128,
+// bfloat16, 32 and 64) query rows of a key/value head per tile; max_rows: those of the largest tree (as far as the host knows).
+// blocks: those that share all keys evenly, in units of `unit` keys (a power of two from 64 on), no block fewer than `least`, a pair
+// `gap` units beside its keys; they need part_o [2 * blocks, tile_rows * dh], part_ml [2 * blocks, tile_rows, 2] and cuts [blocks]
+// (8 integers each).  0: a block for every pair of tile and head.  The head size is a multiple of 16 up to 256.
 // (Packed in 64-bit fields: draft.cu says why.)
 struct TreeAttentionArgs {
     const void *q, *k_pages, *v_pages;

@@ -7,14 +7,13 @@ template <int DP>
 int by_rows(const Args* a, long long pages, int tile_rows, int wide, int* info, cudaStream_t stream) {
     if (tile_rows == 16) {
         if constexpr (DP <= 64) {
-            if (wide == 1) TREE_GO(float, 16, 1, 8, 32, 1, 1);
-            if (wide == 2) TREE_GO(float, 16, 1, 2, 32, 1, 5);
-            if (!wide) TREE_GO(float, 16, 1, 4, 32, 1, 3);
+            if (wide == 1) TREE_GO(float, 1, 8, 32, 1, 1);
+            if (!wide) TREE_GO(float, 1, 4, 32, 1, 3);
         } else if constexpr (DP == 128) {
-            if (wide == 1) TREE_GO(float, 16, 1, 6, 32, 1, 1);
-            if (!wide) TREE_GO(float, 16, 1, 3, 32, 1, 2);
+            if (wide == 1) TREE_GO(float, 1, 6, 32, 1, 1);
+            if (!wide) TREE_GO(float, 1, 3, 32, 1, 2);
         } else {
-            if (!wide) TREE_GO(float, 16, 1, 3, 32, 1, 1);
+            if (!wide) TREE_GO(float, 1, 3, 32, 1, 1);
         }
     }
     return mllm_fail(1, "tree_attention: no kernel takes tiles of %d rows (variant %d)", tile_rows, wide);

@@ -87,7 +87,9 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <typename T, int DP, int RW, int WR, int WK, int BK, int ST>
+constexpr int RW = 16;                                      // query rows of a warp: those of an MMA
+
+template <typename T, int DP, int WR, int WK, int BK, int ST>
 struct Shape {
     static constexpr int VEC = 16 / sizeof(T);
     static constexpr int ROW = DP + VEC;                    // a query row, padded: neighbours start on other banks
@@ -97,7 +99,6 @@ struct Shape {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr size_t q_bytes = (size_t)ROWS * ROW * sizeof(T);
     static constexpr size_t kv_bytes = (size_t)WK * ST * 2 * TILE * sizeof(T);
-    static_assert(RW == 16, "rows of an MMA");
     static constexpr int MN = 2;                            // rows whose maximum and sum a thread keeps
     static constexpr int ON = DP / 2;                       // and its elements of the result
     static constexpr int X_ROW = DP + 8;                    // the groups' results meet as rows of 32-bit floats
@@ -105,10 +106,10 @@ struct Shape {
     static constexpr size_t bytes = (kv_bytes > xch_bytes ? kv_bytes : xch_bytes) + q_bytes;
 };
 
-template <typename T, int DP, int RW, int WR, int WK, int BK, int ST, int PER_SM, bool TMA>
+template <typename T, int DP, int WR, int WK, int BK, int ST, int PER_SM, bool TMA>
 __global__ void __launch_bounds__(WR * WK * 32, PER_SM)
 tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, int box, int pool_rows) {
-    using S = Shape<T, DP, RW, WR, WK, BK, ST>;
+    using S = Shape<T, DP, WR, WK, BK, ST>;
     constexpr int VEC = S::VEC, ROW = S::ROW, CH = DP / VEC, NT = WR * 32, MN = S::MN, ON = S::ON, TILE = S::TILE;
     constexpr bool F32 = S::F32;
     using mask_t = typename std::conditional<BK == 32, uint32_t, unsigned long long>::type;
@@ -570,13 +571,12 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
     }
 }
 
-
-template <typename T, int DP, int RW, int WR, int WK, int BK, int ST, int PER_SM, bool TMA>
+template <typename T, int DP, int WR, int WK, int BK, int ST, int PER_SM, bool TMA>
 int launch(const Args& a, long long pages, cudaStream_t stream) {
-    using Sh = Shape<T, DP, RW, WR, WK, BK, ST>;
+    using Sh = Shape<T, DP, WR, WK, BK, ST>;
     constexpr size_t fixed = 1024;                          // the segments and barriers, up to the alignment of the buffers
     static_assert(Sh::bytes + fixed <= 232448 && (Sh::bytes + fixed + 1024) * PER_SM <= 233472, "shared memory of an SM");
-    auto kern = tree_attention_kernel<T, DP, RW, WR, WK, BK, ST, PER_SM, TMA>;
+    auto kern = tree_attention_kernel<T, DP, WR, WK, BK, ST, PER_SM, TMA>;
     static bool set = false;
     if (!set && Sh::bytes + fixed > 48 * 1024) {
         MLLM_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::bytes));
@@ -597,11 +597,17 @@ int launch(const Args& a, long long pages, cudaStream_t stream) {
 
 // One variant, with copies by TMA where the pages allow it.  info not null: only says how many of its blocks an SM holds, and how many
 // keys a block walks at once.
-#define TREE_GO(T, RW, WR, WK, BK, ST, PER)                                                                         \
+#define TREE_GO(T, WR, WK, BK, ST, PER)                                                                             \
     do {                                                                                                            \
         if (info) { info[0] = PER; info[1] = WK * BK; return 0; }                                                   \
-        return boxes_ok(*a, pages) ? launch<T, DP, RW, WR, WK, BK, ST, PER, true>(*a, pages, stream)                \
-                                   : launch<T, DP, RW, WR, WK, BK, ST, PER, false>(*a, pages, stream);              \
+        return boxes_ok(*a, pages) ? launch<T, DP, WR, WK, BK, ST, PER, true>(*a, pages, stream)                    \
+                                   : launch<T, DP, WR, WK, BK, ST, PER, false>(*a, pages, stream);                  \
+    } while (0)
+// The same for tiles that pages of a multiple of 8 tokens leave to the tcgen05 kernel: copies by the threads only.
+#define TREE_GO_NO_BOXES(T, WR, WK, BK, ST, PER)                                                                    \
+    do {                                                                                                            \
+        if (info) { info[0] = PER; info[1] = WK * BK; return 0; }                                                   \
+        return launch<T, DP, WR, WK, BK, ST, PER, false>(*a, pages, stream);                                        \
     } while (0)
 
 }  // namespace

@@ -118,7 +118,6 @@ def _signatures(lib):
                                  c_void_p, c_ll, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
         "mllm_attention_tiled_wide": [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p,
                                       c_void_p, c_ll, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p],
-        "mllm_draft_max_nodes": [],
         "mllm_draft_tables": [c_char_p, c_void_p],
         "mllm_tree_attention_bind_error": [c_void_p],
         "mllm_tree_attention_error": [c_void_p],
@@ -2443,7 +2442,7 @@ def _tree_variant(float32: bool, head_dim: int, tile: int, wide: int):
 def tree_plan(float32: bool, S: int, num_heads: int, num_kv_heads: int, head_dim: int, max_nodes: int, max_length: int, boxes: bool,
               sms: int):
     """How a tree attention is cut: (query rows of a tile, those of the largest tree, blocks that share the keys evenly (0: one for
-    every pair of tile and key/value head), units that a block takes at least, variant).  ``boxes``: pages come by TMA.
+    every pair of tile and key/value head), units that a block takes at least, variant).  ``boxes``: pages can come by TMA.
 
     Tiles.  float32: 16 rows (more rows are more tiles: keys and values come from L2 again).  bfloat16: 16 on mma.sync while one
     holds a tree's rows, 128 and 256 in tensor memory beyond, where it takes the heads and pages; for heads of up to 64 and up to 64
@@ -2517,7 +2516,7 @@ def tree_attention(q, k_pages, v_pages, block_table, lengths, cu_nodes, ancestor
     words = ancestors.shape[1]
     tile, rows, blocks, least, wide = tree_plan(
         dt == F32, S, num_heads, num_kv_heads, head_dim, min(T, 32 * words if max_nodes is None else int(max_nodes)),
-        width * ps if max_length is None else min(int(max_length), width * ps), ps % 8 == 0, sm_count())
+        width * ps if max_length is None else min(int(max_length), width * ps), ps % 8 == 0 and P * Hkv * ps < 0x7fffff00, sm_count())
     part_o = part_ml = cuts = 0
     if blocks:
         parts = 2 * blocks * tile
