@@ -234,6 +234,19 @@ def test_long_texts_and_wide_trees(ops, dtype, lengths, n, H, Hkv, d, ps):
 
 
 @pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("n,H,Hkv,d,page", [(4, 2, 2, 48, 16), (30, 2, 1, 64, 16), (12, 8, 1, 128, 16), (50, 8, 2, 128, 8), (9, 4, 2, 64, 5)])
+def test_many_short_texts_between_long_ones(ops, dtype, n, H, Hkv, d, page):
+    """Keys shared out where most pairs are shorter than what comes before each of them: pieces that end and begin anywhere, blocks of
+    more segments than fit one list, requests without rows."""
+    rng = random.Random(n + d)
+    lengths = [rng.choice((0, 1, 5, 63, 64, 65, 200)) for _ in range(70)] + [3000, 0, 1500]
+    counts = [rng.choice((0, 1, n // 2, n)) for _ in lengths]
+    counts[70] = n
+    for hints in (dict(max_nodes=n, max_length=100000), dict(max_nodes=n, max_length=3000)):
+        Case(dtype, lengths, counts, H, Hkv, d, page, seed=n + d).check(ops, **hints)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
 def test_hints_only_change_how_the_work_is_cut(ops, dtype):
     for hints in (dict(), dict(max_nodes=20, max_length=700), dict(max_nodes=1, max_length=1), dict(max_nodes=256, max_length=100000)):
         Case(dtype, [700, 3, 128], [20, 5, 1], 4, 2, 32, 16, seed=2).check(ops, **hints)
