@@ -82,8 +82,8 @@ tree_attention_join_kernel(const Args a) {
             }
         }
         const float inv = inverse_sum(l);
-        const int q = cut.row0 + row;
-        T* orow = static_cast<T*>(a.out) + (size_t)(cut.first + q / G) * a.ldo + (size_t)(cut.hk * G + q % G) * a.dh;
+        const int q = cut.row0 + row, node = node_of(a, q);
+        T* orow = static_cast<T*>(a.out) + (size_t)(cut.first + node) * a.ldo + (size_t)(cut.hk * G + q - node * G) * a.dh;
 #pragma unroll
         for (int x = 0; x < VD; ++x)
             if (x * 32 + lane < a.dh) orow[x * 32 + lane] = from_f32<T>(o[x] * inv);
@@ -147,8 +147,8 @@ tree_attention_join_tall_kernel(const Args a) {
             }
         }
         const float inv = inverse_sum(l);
-        const int q = cut.row0 + row;
-        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + (size_t)(cut.first + q / G) * a.ldo + (size_t)(cut.hk * G + q % G) * a.dh + 4 * quad;
+        const int q = cut.row0 + row, node = node_of(a, q);
+        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + (size_t)(cut.first + node) * a.ldo + (size_t)(cut.hk * G + q - node * G) * a.dh + 4 * quad;
 #pragma unroll
         for (int x = 0; x < 4; ++x) to[x] = __float2bfloat16(o[x] * inv);
     }
@@ -263,7 +263,7 @@ MLLM_EXPORT int mllm_tree_attention(const TreeAttentionArgs* p, cudaStream_t str
     while (out_vec < 8 && (uintptr_t)p->out % (2 * out_vec * es) == 0 && p->ldo % (2 * out_vec) == 0) out_vec *= 2;
     const Args a{p->q, p->ldq, p->k_pages, p->v_pages, p->block_table, (int)p->bt_stride, (int)p->width, p->lengths, p->cu_nodes, p->ancestors,
                  (int)p->words, p->out, p->ldo, p->part_o, p->part_ml, p->cuts, (int)p->S, H, Hkv, H / Hkv, dh, page_size,
-                 shifts ? 31 - __builtin_clz(page_size) : -1, (uintptr_t)p->q % 16 == 0 && p->ldq * es % 16 == 0, out_vec, tile_rows,
+                 shifts ? 31 - __builtin_clz(page_size) : -1, ((1ULL << 32) + H / Hkv - 1) / (H / Hkv), (uintptr_t)p->q % 16 == 0 && p->ldq * es % 16 == 0, out_vec, tile_rows,
                  31 - __builtin_clz(tile_rows), (int)(p->max_rows < tile_rows ? p->max_rows : tile_rows), 31 - __builtin_clz((int)p->unit), (int)p->least, (int)p->blocks, (int)p->gap,
                  (int)max_tiles, scale * LOG2E};
     if (dtype == MLLM_F32) return tree::f32(&a, dh, p->pages, tile_rows, (int)p->wide, nullptr, stream);

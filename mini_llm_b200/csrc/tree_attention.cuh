@@ -16,13 +16,17 @@ struct Args {
     void* out; long long ldo;
     float* part_o; float* part_ml;          // [2 * blocks, tile rows, dh] (tree_attention.cu says in what order) and [2 * blocks, tile rows, 2]
     struct Cut* cuts;                       // [blocks]
-    int S, H, Hkv, G, dh, page_size, page_shift;
+    int S, H, Hkv, G, dh, page_size, page_shift;       // shift: -1 where it is no power of two
+    unsigned long long g_inverse;           // 2^32 / G, rounded up
     int q_vec, out_vec;                     // queries can be read 16 bytes at a time; elements that a store may write at once
     int tile_rows, tile_shift, max_rows;    // query rows of a tile (a power of two), and those of the largest tree's first
     int unit_shift, least, blocks, gap;     // keys per unit of work, the least of them for a block, blocks (0: one per pair), a pair's own cost in units
     int max_tiles;
     float scale_log2;
 };
+
+// The node of query row r, r / G: the inverse is too large by less than G / 2^32, so the quotient is right for r * G < 2^32.
+__device__ __forceinline__ int node_of(const Args& a, int r) { return (int)((unsigned int)r * a.g_inverse >> 32); }
 
 // A pair of query rows and head that the boundary before block c cuts, if no earlier boundary does (else parts is 0): where its rows
 // go, and whose sums they are.  Block c writes it, the join kernel reads it.

@@ -307,8 +307,8 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                     const int e = threadIdx.x + (i0 + i) * (P::SOFTMAX_WARPS * 32), row = e / (DP / 8), c = e % (DP / 8);
                     v[i] = make_uint4(0u, 0u, 0u, 0u);
                     if (row >= rows || c * 8 >= a.dh) continue;
-                    const bf* src = static_cast<const bf*>(a.q) + (size_t)(sg.first + (sg.row0 + row) / G) * a.ldq +
-                                    (size_t)(sg.hk * G + (sg.row0 + row) % G) * a.dh + c * 8;
+                    const int q = sg.row0 + row, node = tree::node_of(a, q);
+                    const bf* src = static_cast<const bf*>(a.q) + (size_t)(sg.first + node) * a.ldq + (size_t)(sg.hk * G + q - node * G) * a.dh + c * 8;
                     if (a.q_vec) {
                         v[i] = *reinterpret_cast<const uint4*>(src);
                     } else {
@@ -330,8 +330,9 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
             const int steps = steps_of(sg, ks);
             const int tile_row = qt * BQ + r;                 // row among the block's tiles
             const bool active = qt * BQ + q4 * 32 < rows;
-            const int node = tile_row < rows ? (sg.row0 + tile_row) / G : 0;
-            const int* words = a.ancestors + (size_t)(sg.first + node) * a.words;
+            // (found again where they are needed: registers that the softmax has no room for)
+            auto node_here = [&]() { return tile_row < rows ? tree::node_of(a, sg.row0 + tile_row) : 0; };
+            auto words_here = [&]() { return a.ancestors + (size_t)(sg.first + node_here()) * a.words; };
             const int tail_from = min(sg.len, sg.keys);   // from here on rows do not all see what is there
             float m_run = -INFINITY, l_run = 0.f;
             for (int i = 0; i < steps; ++i, ++it) {
@@ -339,7 +340,7 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                 const bool tail = key0 + BKV > tail_from;
                 unsigned long long seen = ~0ull;
                 if (tail) {
-                    if (active) seen = tree::tile_mask(words, a.words, sg.len, sg.keys, key0, tile_row < rows);
+                    if (active) seen = tree::tile_mask(words_here(), a.words, sg.len, sg.keys, key0, tile_row < rows);
                     // values past the last key and those that are not finite: out, before the product reads them
                     const int s = it % STAGES;
                     bool got = mbar_wait(&bars.v_full[ks][s], (it / STAGES) & 1);
@@ -458,27 +459,31 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                     f[y] = my == -INFINITY ? 0.f : tree::fast_exp2((my - m) * sl2);
                     l = fmaf(f[y], sm_l[(y * QT + qt) * BQ + r], l);
                 }
-                const int q = sg.row0 + tile_row;
+                const int q = sg.row0 + tile_row, node = node_here();
+                const int* words = words_here();
                 const float inv = tree::inverse_sum(l);
                 const size_t slot = max(sg.slot, 0);
                 if (sg.slot >= 0 && tile_row < rows && ks == 0)
                     *reinterpret_cast<float2*>(a.part_ml + 2 * (slot * a.tile_rows + tile_row)) = make_float2(m, l);
-                bf* orow = static_cast<bf*>(a.out) + (size_t)(sg.first + node) * a.ldo + (size_t)(sg.hk * G + q % G) * a.dh;
+                bf* orow = static_cast<bf*>(a.out) + (size_t)(sg.first + node) * a.ldo + (size_t)(sg.hk * G + q - node * G) * a.dh;
 #pragma unroll 1
                 for (int c0 = ks * (DP / KS); c0 < (ks + 1) * (DP / KS) && c0 < a.dh; c0 += 16) {
                     float o[16];
-                    uint32_t w[KS][16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[e] = 0.f;
+                    constexpr int Y = KS < 2 ? KS : 2;                // streams at a time
 #pragma unroll
-                    for (int y = 0; y < KS; ++y)
-                        tmem_ld16_issue(tmem + P::TMEM_O + t_lane + (uint32_t)((y * QT + qt) * DP + c0), w[y]);
-                    tmem_ld_wait();
+                    for (int y0 = 0; y0 < KS; y0 += Y) {
+                        uint32_t w[Y][16];
 #pragma unroll
-                    for (int y = 0; y < KS; ++y) {
-                        if (steps_of(sg, y) == 0) continue;           // uniform: the stream's columns were not written
+                        for (int y = 0; y < Y; ++y) tmem_ld16_issue(tmem + P::TMEM_O + t_lane + (uint32_t)(((y0 + y) * QT + qt) * DP + c0), w[y]);
+                        tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = fmaf(f[y], __uint_as_float(w[y][e]), o[e]);
+                        for (int y = 0; y < Y; ++y) {
+                            if (steps_of(sg, y0 + y) == 0) continue;  // uniform: the stream's columns were not written
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = fmaf(f[y0 + y], __uint_as_float(w[y][e]), o[e]);
+                        }
                     }
                     if (tile_row >= rows) continue;
                     if (*odd_seen) {                                  // values that are not finite, to the rows that see them

@@ -224,7 +224,7 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
         for (int i = threadIdx.x; i < S::ROWS * CH; i += WR * WK * 32) {
             const int r = i / CH, c = i % CH;
             const bool ok = r0 + r < rows && c < dh_ch;
-            const int node = ok ? (r0 + r) / G : 0, h = hk * G + (ok ? (r0 + r) % G : 0);
+            const int node = ok ? node_of(a, r0 + r) : 0, h = hk * G + (ok ? r0 + r - node * G : 0);
             const T* src = q + (size_t)(first + node) * a.ldq + (size_t)h * a.dh + c * VEC;
             if (a.q_vec) {
                 cp_async16(sQ + r * ROW + c * VEC, ok ? src : q, ok);
@@ -271,7 +271,7 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
             for (int ks = 0; ks < DP / 16; ++ks) ldsm_x4(qa[ks], s_u32(sQ + (warp * 16 + (lane & 15)) * ROW + ks * 16 + (lane >> 4) * 8));
         }
         auto row_of = [&](int i) { return r0 + warp * RW + g + 8 * i; };      // the query row of a thread's i-th state
-        auto words_of = [&](int r) { return a.ancestors + (size_t)(first + (r < rows ? r / G : 0)) * a.words; };
+        auto words_of = [&](int r) { return a.ancestors + (size_t)(first + (r < rows ? node_of(a, r) : 0)) * a.words; };
 
         for (int use = TMA ? uses : 0; t <= t_last; t += WK, ++use) {
             const int stage = use % ST;
@@ -503,7 +503,8 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
                 return;
             }
             const float inv = inverse_sum(l);
-            T* orow = static_cast<T*>(a.out) + (size_t)(first + r / G) * a.ldo + (size_t)(hk * G + r % G) * a.dh;
+            const int node = node_of(a, r);
+            T* orow = static_cast<T*>(a.out) + (size_t)(first + node) * a.ldo + (size_t)(hk * G + r - node * G) * a.dh;
             if (F32 && a.out_vec >= 2) *reinterpret_cast<float2*>(orow + d) = make_float2(x * inv, y * inv);
             else if (!F32 && a.out_vec >= 2) *reinterpret_cast<uint32_t*>(orow + d) = pack_bf16(x * inv, y * inv);
             else { orow[d] = from_f32<T>(x * inv); orow[d + 1] = from_f32<T>(y * inv); }

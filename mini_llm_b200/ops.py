@@ -2506,6 +2506,8 @@ def tree_attention(q, k_pages, v_pages, block_table, lengths, cu_nodes, ancestor
         raise KernelError("tree_attention: head counts or sizes do not fit the pages")
     if head_dim % 16 != 0 or not (16 <= head_dim <= 256):
         raise KernelError(f"tree_attention: head size {head_dim} is not a multiple of 16 in 16..256")
+    if T * (num_heads // num_kv_heads) ** 2 >= 1 << 32:
+        raise KernelError(f"tree_attention: {T} rows of {num_heads // num_kv_heads} heads per key/value head are more than 32-bit numbers hold")
     n_tables, width = block_table.shape
     if n_tables != S:
         raise KernelError(f"tree_attention: block_table {tuple(block_table.shape)} for {S} requests")
