@@ -14,6 +14,7 @@ The reference decodes one token per request and call (src/model/gpt2_model.cu:45
 """
 from __future__ import annotations
 
+import itertools
 from collections import deque
 from dataclasses import dataclass, field
 from typing import Dict, Hashable, List, Optional, Sequence, Tuple
@@ -96,9 +97,12 @@ class DraftStats:
     tokens: int = 0            # tokens that came of them
 
 
+_buffers = itertools.count(1)
+
+
 class _TreeLayout:
-    def __init__(self, T: int, S: int, max_pages: Tuple[int, ...], words: int, rows: int):
-        self._key = (T, S, T, max_pages, "tree", words, rows)
+    def __init__(self, T: int, S: int, max_pages: Tuple[int, ...], words: int, rows: int, depth: int, buffers: int):
+        self._key = (T, S, T, max_pages, "tree", words, rows, depth, buffers)
 
     def key(self):
         return self._key
@@ -133,14 +137,15 @@ class DraftRunner:
         self.words = -(-self.rows // 32)
         self._host: List[Optional[torch.Tensor]] = [None, None]
         self._dev: Optional[torch.Tensor] = None
+        self._buffers = 0         # which device buffer this is, of all that such runners ever had: captured graphs hold its address
 
     def _ints(self, n: int) -> Tuple[torch.Tensor, torch.Tensor]:
-        """(pinned host buffer, device buffer) of at least n 32-bit words; captured graphs are dropped when the latter moves."""
+        """(pinned host buffer, device buffer) of at least n 32-bit words; graphs captured with an earlier one are not met again."""
         if self._dev is None or self._dev.numel() < n:
             cap = max(1 << 14, 1 << (n - 1).bit_length())
             self._host = [torch.empty(cap, dtype=torch.int32, pin_memory=True) for _ in range(2)]
             self._dev = torch.zeros(cap, dtype=torch.int32, device=self.runner.device)
-            self.runner.ws.version += 1
+            self._buffers = next(_buffers)
         return self._host[0], self._dev
 
     def step(self, entries: Sequence[DraftEntry]) -> List[DraftResult]:
@@ -243,7 +248,7 @@ class DraftRunner:
             groups.append(GroupView(block_table=table, slot_mapping=slots, max_pages=widths[g]))
         ctx = DraftContext(T=T, S=S, R=T, ws=r.ws, token_ids=view("tokens"), positions=view("positions"), token_seq=view("seq"),
                            logit_rows=view("rows"), state_slots=None, q_start=lengths, ctx_len=view("ctx_len"), cu_q=cu, groups=groups,
-                           layout=_TreeLayout(T, S, widths, self.words, R), max_q_len=R, max_ctx_len=deepest + R,
+                           layout=_TreeLayout(T, S, widths, self.words, R, depth, self._buffers), max_q_len=R, max_ctx_len=deepest + R,
                            q_lens=[R] * S, q_starts=[cm.computed(e.req) for e in entries],
                            tree=TreeView(lengths=lengths, cu_nodes=cu, ancestors=ancestors, max_nodes=R,
                                          max_length=ops.split_context(deepest + R)))
@@ -280,7 +285,10 @@ class DraftedDecoder:
 
     def __init__(self, llm, drafter=None, rows: int = 16, depth: int = 8):
         self.llm, self.runner, self.drafter = llm, llm.runner, drafter if drafter is not None else PromptLookup()
-        self.trees = DraftRunner(llm.runner, rows, depth)
+        # the last call's, where it fits: its steps are captured graphs already
+        if llm.draft_runner is None or (llm.draft_runner.rows, llm.draft_runner.depth) != (int(rows), int(depth)):
+            llm.draft_runner = DraftRunner(llm.runner, rows, depth)
+        self.trees = llm.draft_runner
         self.stats = DraftStats()
 
     def _done(self, req: Request) -> bool:

@@ -34,6 +34,7 @@ class LLM:
         self._inflight = None          # (advanced step, sampler ticket, request id -> row) of a step whose tokens are not read yet
         self._held: List[Response] = []     # responses read while aborting, handed out by the next step()
         self.metrics = ServingMetrics()      # arrival, first and last token of every request (host clock)
+        self.draft_runner = None             # of the last generate_drafted: its buffers and captured steps
         self.draft_stats = None              # of the last generate_drafted: passes, trees and the tokens that came of them
         self.profile = None                  # a list: step() then times every launch and appends a row per kernel
         self._profile_steps = 0

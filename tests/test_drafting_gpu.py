@@ -150,6 +150,43 @@ def test_steps_of_one_shape_are_replayed_as_graphs(setup):
     assert llm.draft_stats.steps > 5 and llm.runner.graph_replays >= llm.draft_stats.steps - 4
 
 
+def test_steps_stay_graphs_from_call_to_call(setup):
+    """A second call replays what the first one captured; one with other rows or depths, or steps of plain decoding in between, changes
+    neither call's tokens."""
+    import mini_llm_b200 as m
+    prompts = [random_ids(9, setup["cfg"]["vocab_size"], s) for s in (3, 4)]
+    sp = m.SamplingParams(max_new_tokens=20, ignore_eos=True)
+    llm = make(setup)
+    want = [llm.generate_drafted(prompts, sp, rows=8, depth=d) for d in (4, 8)]
+    for _ in range(3):
+        llm.generate(prompts, sp)
+    for d, w in ((8, want[1]), (8, want[1]), (4, want[0]), (4, want[0]), (8, want[1])):
+        assert llm.generate_drafted(prompts, sp, rows=8, depth=d) == w
+    before = llm.runner.graph_replays
+    assert llm.generate_drafted(prompts, sp, rows=8, depth=8) == want[1]
+    assert llm.runner.graph_replays - before >= llm.draft_stats.steps
+
+
+def test_two_runners_of_trees_on_one_model(setup):
+    """Each has buffers of its own: the one's captured steps are not the other's, whatever they have in common."""
+    from mini_llm_b200.engine.drafting import DraftEntry, DraftRunner
+    from mini_llm_b200.engine.runner import StepEntry
+    got = {}
+    for order in ("one", "both"):
+        llm = make(setup)
+        r = llm.runner
+        runners = [DraftRunner(r, 4, 4) for _ in range(2)]
+        r.add_request("q")
+        r.step([StepEntry("q", random_ids(7, setup["cfg"]["vocab_size"], 5), ())])
+        out, last = [], 1
+        for i in range(12):
+            res = runners[i % 2 if order == "both" else 0].step([DraftEntry("q", [last, last, 2, 3], [-1, 0, 1, 2])])[0]
+            out += res.tokens
+            last = res.tokens[-1]
+        got[order] = out
+    assert got["one"] == got["both"]
+
+
 def test_refusals(setup, tmp_path):
     import mini_llm_b200 as m
     from mini_llm_b200.engine.drafting import DraftEntry, DraftRunner
