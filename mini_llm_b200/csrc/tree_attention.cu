@@ -155,8 +155,10 @@ tree_attention_join_tall_kernel(const Args a) {
 }
 int launch_join_tall(const Args& a, cudaStream_t stream) {
     if (a.blocks < 2) return 0;
-    if (a.dh <= 64) MLLM_CUDA(mllm_launch(tree_attention_join_tall_kernel<16>, dim3(a.blocks - 1, (a.max_rows + 15) / 16), dim3(256), 0, stream, true, a));
-    else MLLM_CUDA(mllm_launch(tree_attention_join_tall_kernel<8>, dim3(a.blocks - 1, (a.max_rows + 7) / 8), dim3(256), 0, stream, true, a));
+    // most boundaries cut nothing that an earlier one does not: no more blocks than are resident at once, several rows a thread
+    const int rows = a.dh <= 64 ? 16 : 8, y = min((a.max_rows + rows - 1) / rows, 8);
+    if (a.dh <= 64) MLLM_CUDA(mllm_launch(tree_attention_join_tall_kernel<16>, dim3(a.blocks - 1, y), dim3(256), 0, stream, true, a));
+    else MLLM_CUDA(mllm_launch(tree_attention_join_tall_kernel<8>, dim3(a.blocks - 1, y), dim3(256), 0, stream, true, a));
     return 0;
 }
 
