@@ -293,14 +293,31 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
         const unsigned long long sl2_2 = pack2(sl2, sl2);
         int it = 0, done = 0;                                 // blocks, commits to o_full so far
         bool alive = true;
+        // One tile: the next segment's queries are asked for while this one's sums are read (cp.async, which takes no registers)
+        constexpr bool AHEAD = QT == 1 && KS > 1;
+        bool asked = false;
+        auto ask = [&](const Segment& sg) {
+            const int rows = sg.rows - sg.row0;
+#pragma unroll
+            for (int i = 0; i < P::Q_PIECES; ++i) {
+                const int e = threadIdx.x + i * (P::SOFTMAX_WARPS * 32), row = e / (DP / 8), c = e % (DP / 8);
+                if (row >= rows) continue;
+                const int q = sg.row0 + row, node = tree::node_of(a, q), n = c * 8 < a.dh ? 16 : 0;      // no bytes: zeros
+                const bf* src = static_cast<const bf*>(a.q) + (n ? (size_t)(sg.first + node) * a.ldq + (size_t)(sg.hk * G + q - node * G) * a.dh + c * 8 : 0);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(sQ + (c >> 3) * (BQ * 128) + row * 128 + ((c ^ row) & 7) * 16)),
+                             "l"(src), "r"(n) : "memory");
+            }
+            asked = true;
+        };
         do {
         for (int n = 0; alive && n < segments->count; ++n) {
             const Segment& sg = segments->list[n];
             const int rows = sg.rows - sg.row0;               // query rows of the block's tiles
             // ---- the queries, 16-byte pieces, up to eight of a thread's in flight; rows past the end are never looked at
             constexpr int BATCH = P::Q_PIECES < 8 ? P::Q_PIECES : 8;
+            if (AHEAD && asked) asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
-            for (int i0 = 0; i0 < P::Q_PIECES; i0 += BATCH) {
+            for (int i0 = AHEAD && asked ? P::Q_PIECES : 0; i0 < P::Q_PIECES; i0 += BATCH) {
                 uint4 v[BATCH];
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i) {
@@ -323,6 +340,7 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                         *reinterpret_cast<uint4*>(sQ + (row / BQ) * P::Q_BYTES + (c >> 3) * (BQ * 128) + (row % BQ) * 128 + ((c ^ row) & 7) * 16) = v[i];
                 }
             }
+            asked = false;
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.q_full);
@@ -447,6 +465,8 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
             sm_l[x * BQ + r] = l_run;
             if (KS > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + qt * 4 + q4), "n"(KS * 32) : "memory");
             else __syncwarp();
+            // every stream's last scores are done (its warp here has read them), so nothing reads this segment's queries any more
+            if (AHEAD && alive && a.q_vec && n + 1 < segments->count) ask(segments->list[n + 1]);
             if (alive && active) {
                 tc_fence_after();
                 float m = -INFINITY, l = 0.f;
@@ -535,6 +555,7 @@ tree_attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
     __syncthreads();
     if (*failed) {
         if (threadIdx.x == 0) { atomicCAS(&g_tree_error, 0, *failed); report_to_host(1000 + *failed); }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         for (int i = 0; i < 2000; ++i) __nanosleep(100);          // copies and MMAs already issued may still be running
         __syncthreads();
     }
