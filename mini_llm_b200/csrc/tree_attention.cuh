@@ -36,7 +36,7 @@ struct Cut { int parts, first, hk, row0, rows, slot, shift, unused; };      // s
 // A pair is a tile of query rows of one (request, key/value head).  Either every pair has a block of its own (blocks == 0: the grid
 // is (head and tile, request)), or the pairs' keys are shared out evenly: each pair's keys in units of 2^unit_shift, all units of all pairs
 // in one line, in order of request, head, tile and position, before each pair's a gap for what the pair costs beside its keys (without
-// gaps, blocks that got many short texts held up the rest: 24 requests of 200 to 3,000 keys, 12 heads, 40 rows: 95 us, with them 56).
+// gaps, blocks that got many short texts held up the rest: 24 requests of 200 to 3,000 keys, 12 heads, 40 rows: 95 us, with them 56, and 52 since).
 // Every block takes as long a piece of that line as any other (or one unit less), whatever the lengths, but no fewer units than its
 // groups or streams can walk at once.  A block's share of one pair is a segment.  Pairs that lie in one block are finished there; the
 // others leave their segments' sums in scratch, two slots a block (only its first and last segment can be parts of a pair), and the

@@ -2453,8 +2453,8 @@ def tree_plan(float32: bool, S: int, num_heads: int, num_kv_heads: int, head_dim
     Blocks.  A round is what a block walks at once.  A block per pair takes as many as the longest request, times the waves of
     pairs; sharing the keys out evenly takes their sum, and the join.  Variants differ in groups per block: 1, more groups for few
     pairs, 2, fewer for many blocks.  12 pairs of 518 keys: 9.2 us in wide blocks, 10.7 in others, 10.7 shared; 192 pairs of up to
-    1,008: 14.6 in blocks of their own, 17.0 shared; 64 pairs of up to 8,004 (heads of 128): 112 and 40.  Over 104 shapes the variant
-    that this picks took 1.4 % more than the fastest, and 15 % at most."""
+    1,008: 14.6 in blocks of their own, 17.0 shared; 64 pairs of up to 8,004 (heads of 128): 112 and 40.  Over 129 shapes the variant
+    that this picks took 1.4 % more than the fastest, and 17 % at most."""
     rows = max(1, max_nodes * (num_heads // num_kv_heads))
     if float32 or rows <= 16:
         tiles = (16,)
