@@ -102,7 +102,7 @@ int launch_join(const Args& a, cudaStream_t stream) {
 
 // The same for the tiles of the tcgen05 kernel, whose threads hold a row each: sums lie four columns of all rows at a time
 // ([slot][columns / 4][row][4]), so that a warp's 32 rows are 512 neighbouring bytes where it writes them (as rows, 32 pieces of 16
-// bytes in lines of their own: 256 rows of 128, 8 us a block).  A thread takes four columns of a row, R rows a block.
+// bytes in lines of their own: 256 rows of 128, 8,600 cycles a block where this takes 4,800).  A thread takes four columns of a row, R rows a block.
 template <int R>
 __global__ void __launch_bounds__(256)
 tree_attention_join_tall_kernel(const Args a) {
