@@ -21,13 +21,13 @@
 // for every 512 bytes).  The groups meet in order at the end.
 //   bfloat16: S = Q K^T and O += P V on mma.sync.m16n8k16, p as two bfloat16 terms (its rounding and what that left out), so the
 //             weights keep about 16 bits; sums in 32 bits.  (Products of two or eight rows on tcgen05 would be 128 high.)
-//   float32:  on mma.sync.m16n8k8 with both factors as two 11-bit terms, three products of the four: sums of the large ones in two
-//             chains, of the mixed ones in a third; a tile's sums of P V by themselves, added rounded.  Fused multiply-adds on the
-//             CUDA cores took 121 us where this takes 106 (below).
+//   float32:  on mma.sync.m16n8k8 with both factors as two 11-bit terms, three products of the four: the large ones
+//             summed 32 columns (or keys) at a time and added rounded, the mixed ones by themselves.  Fused multiply-adds on the
+//             CUDA cores took 121 us where this takes 105 (below).
 // Measured (one launch among others, the join's included; what the bytes take at 6.5 TB/s in brackets): bfloat16, 12 heads of 64:
 // 1 request, 8 rows, 510 keys 8.7 us (0.2); 8 requests, 32 rows, up to 990 keys 14.1 us (2.7); 64 requests, up to 48 rows over 4
 // key/value heads, 500 to 4,000 keys 60 us (23; tree_attention_tcgen05.cu takes these, in 56); float32: 8 requests, 16 rows, up to
-// 1,000 keys 22 us (5.0); 5 requests, up to 37 rows, up to 7,001 keys, 25 heads 106 us (41).
+// 1,000 keys 22 us (5.0); 5 requests, up to 37 rows, up to 7,001 keys, 25 heads 105 us (41).
 // Values in places that some rows see and others do not (the tree's own) may be infinite or NaN: a weight of zero would turn them
 // into NaN, so such elements are taken out of the tile and added to the rows that see them only.
 #include "tree_attention_tiles.cuh"

@@ -309,19 +309,25 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
                         }
                     }
                 } else {
-                    // ---- S: three of the four products of terms, the small ones in sums of their own; the large ones in two, since
-                    // the unit cuts its sums off where the CUDA cores round them
-                    float c0[BK / 8][4], c1[BK / 8][4], cs[BK / 8][4];
+                    // ---- S: three of the four products of terms, the small ones in sums of their own; the large ones 32 columns at a
+                    // time, added rounded, since the unit cuts its sums off (two chains over all columns: up to 2.6 times the error of
+                    // plain 32-bit sums for heads of 256, now up to 1.4; heads of 64 107 us -> 105, of 256 75 -> 77)
+                    float cs[BK / 8][4];
 #pragma unroll
                     for (int nt = 0; nt < BK / 8; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) c0[nt][e] = c1[nt][e] = cs[nt][e] = 0.f;
+                        for (int e = 0; e < 4; ++e) sc[4 * nt + e] = cs[nt][e] = 0.f;
                     const uint32_t lk = oK + g * 128 + (g << 4) + tq * 4;
-#pragma unroll(DP <= 64 ? DP / 16 : 4)
-                    for (int k2 = 0; k2 < DP / 16; ++k2)
+#pragma unroll(DP <= 64 ? DP / 32 : 2)
+                    for (int k4 = 0; k4 < DP / 32; ++k4) {
+                        float c0[BK / 8][4];
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const int ks = 2 * k2 + half;
+                        for (int nt = 0; nt < BK / 8; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) c0[nt][e] = 0.f;
+#pragma unroll
+                        for (int part = 0; part < 4; ++part) {
+                            const int ks = 4 * k4 + part;
                             uint32_t ah[4], al[4];
                             split_queries(ks, ah, al);
 #pragma unroll
@@ -329,15 +335,20 @@ tree_attention_kernel(const Args a, const __grid_constant__ CUtensorMap map_k, c
                                 uint32_t bh0, bl0, bh1, bl1;
                                 split_tf32(*reinterpret_cast<const float*>(smem + piece_of(lk, 2 * ks) + nt * 1024), bh0, bl0);
                                 split_tf32(*reinterpret_cast<const float*>(smem + piece_of(lk, 2 * ks + 1) + nt * 1024), bh1, bl1);
-                                mma_tf32(half ? c1[nt] : c0[nt], ah, bh0, bh1);
+                                mma_tf32(c0[nt], ah, bh0, bh1);
                                 mma_tf32(cs[nt], ah, bl0, bl1);
                                 mma_tf32(cs[nt], al, bh0, bh1);
                             }
                         }
 #pragma unroll
+                        for (int nt = 0; nt < BK / 8; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) sc[4 * nt + e] += c0[nt][e];
+                    }
+#pragma unroll
                     for (int nt = 0; nt < BK / 8; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[4 * nt + e] = (c0[nt][e] + c1[nt][e]) + cs[nt][e];
+                        for (int e = 0; e < 4; ++e) sc[4 * nt + e] += cs[nt][e];
                 }
             }
             group_sync<WR>(group);                            // the keys' buffer is free
